@@ -408,6 +408,93 @@ int pb_sample_top_p_host_settings(const void* logits, int32_t dtype, int32_t num
                                   const float* h_temperature, const float* h_top_p, const float* uniforms, int64_t* ids,
                                   void* stream);
 
+/*
+ * ---- The paged cache in 8 bits ----
+ * K and V are held as e4m3 (4 exponent bits, 3 of mantissa, largest value 448, no infinities) with one fp32 scale for
+ * each block and kv head: an element stands for code * scale. Layout as for the other types, with x = 16:
+ *   K: [num_blocks, num_kv_heads, head_size/16, block_size, 16]   V: [num_blocks, num_kv_heads, head_size, block_size]
+ *   scales: [num_blocks, num_kv_heads] fp32, strides in elements, the same for key_scale and value_scale.
+ * Scales are >= 0; 0 says that the whole tile is zero. Head sizes 64, 80, 96, 112, 128, 256; block sizes 16 and 32.
+ * Strides of the caches count elements, which are bytes here, and are multiples of 16.
+ */
+typedef struct pb_fp8_cache {
+  void* key_cache;
+  void* value_cache;
+  float* key_scale;
+  float* value_scale;
+  int64_t kv_block_stride;
+  int64_t kv_head_stride;
+  int64_t scale_block_stride;
+  int64_t scale_head_stride;
+  int64_t num_blocks;
+  int32_t num_kv_heads;
+  int32_t head_size;
+  int32_t block_size;
+} pb_fp8_cache;
+
+/*
+ * KV fill into the 8-bit cache: pb_reshape_and_cache that quantises. For every block b that receives tokens, and every
+ * head, K and V each on their own:
+ *   need  = the smallest power of two with max |x| <= 448 * need over the new tokens' finite elements (0 for all zero)
+ *   old   = 0 if offset 0 of the block is among the new tokens (the block begins anew), else its scale
+ *   scale = max(old, need); new cells = e4m3(x / scale), to nearest even; NaN and infinities are stored as NaN
+ *   the block's other cells are re-quantised, e4m3(c * old / scale), only when the scale grew (exact but for values that
+ *   leave the normal range of e4m3, as long as both scales are powers of two)
+ * Tokens of a block may stand anywhere in slot_mapping; of tokens with the same slot the last in the list counts. A
+ * negative slot, or one outside the cache, skips its token. Rows are fp32, fp16 or bf16 (dtype).
+ * workspace: pb_fp8_fill_workspace_bytes(num_tokens, num_blocks, block_size) bytes of scratch, contents irrelevant.
+ */
+size_t pb_fp8_fill_workspace_bytes(int64_t num_tokens, int64_t num_blocks, int32_t block_size);
+int pb_fp8_reshape_and_cache(const pb_fp8_cache* cache, const void* key, const void* value, const void* slot_mapping,
+                             int32_t slot_is_i64, int64_t num_tokens, int64_t key_stride, int64_t value_stride,
+                             int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows out of the 8-bit cache: code * scale in fp32, rounded once to the rows' type. A token with a negative slot, or
+ * one outside the cache, leaves its rows as they were. */
+int pb_fp8_gather_cached_kv(const pb_fp8_cache* cache, void* key, void* value, const void* slot_mapping,
+                            int32_t slot_is_i64, int64_t num_tokens, int64_t key_stride, int64_t value_stride,
+                            int32_t dtype, void* stream);
+
+/*
+ * pb_attn_plan / pb_shared_prefix_attention_planned / pb_shared_prefix_attention over the 8-bit cache. `p` describes the
+ * problem as there; its key_cache, value_cache, kv_block_stride, kv_head_stride and num_blocks are not read (the cache
+ * brings them), num_kv_heads, head_size and block_size have to be the cache's, and it brings no new tokens
+ * (slot_mapping, key_new and value_new are NULL: the fill is a call of its own). p->dtype is the type of query and out.
+ * Lists planned by one family of entry points are not valid for the other.
+ */
+int pb_fp8_attn_plan(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream);
+int pb_fp8_attention_planned(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream);
+int pb_fp8_attention(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream);
+
+/*
+ * What an iteration's calls read, from the requests' lengths, without the host: blocks for the new tokens, and for every
+ * new token its slot, position and what it attends.
+ *   request r (0 <= r < num_requests) holds context_lens[r] tokens in the first ceil(context_lens[r] / block_size)
+ *   blocks of its table row and adds new_lens[r]. The blocks it lacks are the next ones of free_blocks[0 .. num_free),
+ *   from entry *free_head on, in the order of the requests, and are written into its row of block_tables. Entries of the
+ *   row behind them keep what they held.
+ *   A request whose tokens do not fit its table row, or for which free_blocks runs out, gets nothing: its tokens' slots
+ *   are -1, its kv_lens entry stays context_lens[r], and *num_failed counts it. (Once the list is too short for a request, all later
+ *   ones that need a block fail too; those whose tokens fit the blocks they hold do not.)
+ * Rows are the new tokens of all requests in order; num_tokens rows are written. Row t is token i of request r:
+ *   slot_mapping[t] = table[r][p / block_size] * block_size + p % block_size with p = context_lens[r] + i
+ *   positions[t]    = p + prefix_lens[r]   (prefix_lens NULL: 0)
+ *   requests below num_prefills are causal segments: suffix_lens[t] = 0. For the others suffix_lens[t] = p + 1 and
+ *   suffix_tables[t] = the request's blocks. Entries of suffix_tables[t] beyond the row's blocks are 0.
+ *   rows behind the last token: slot -1, position 0, suffix length 0.
+ * row_offsets [num_requests + 1]: first row of every request (its first num_prefills + 1 entries are seg_row_offsets);
+ * kv_lens [num_requests]: tokens held afterwards (the first num_prefills entries are seg_kv_lens);
+ * *free_head_out: entries of free_blocks taken so far. Only block_tables is changed in place, so the call can be repeated.
+ * suffix_tables may be NULL. Negative lengths count as 0. workspace: pb_block_tables_workspace_bytes(num_requests) bytes.
+ */
+size_t pb_block_tables_workspace_bytes(int32_t num_requests);
+int pb_build_block_tables(const int32_t* context_lens, const int32_t* new_lens, int32_t num_requests, int32_t* block_tables,
+                          int32_t table_width, int64_t table_stride, const int32_t* free_blocks, int32_t num_free,
+                          const int32_t* free_head, const int32_t* prefix_lens, int32_t block_size, int32_t num_prefills,
+                          int64_t num_tokens, int64_t* slot_mapping, int64_t* positions, int32_t* row_offsets,
+                          int32_t* kv_lens, int32_t* suffix_lens, int32_t* suffix_tables, int32_t* free_head_out,
+                          int32_t* num_failed, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,16 @@ from .ops import (  # noqa: F401
     vllm_reshape_and_cache,
     vllm_rotary_emb,
 )
+from .fp8 import (  # noqa: F401
+    Fp8AttentionCall,
+    fp8_flash_paged_attention,
+    fp8_flash_paged_attention_grouped,
+    fp8_gather_cached_kv,
+    fp8_kv_cache,
+    fp8_paged_attention,
+    fp8_reshape_and_cache,
+)
+from .tables import BlockTables, build_block_tables  # noqa: F401
 from . import attention_ops, cache_ops  # noqa: F401
 from .sampler import Sampler  # noqa: F401
 

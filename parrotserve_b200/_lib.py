@@ -105,6 +105,25 @@ class PbHostStep(C.Structure):
     ]
 
 
+class PbFp8Cache(C.Structure):
+    """Mirror of ``pb_fp8_cache`` (same field order as the header)."""
+
+    _fields_ = [
+        ("key_cache", C.c_void_p),
+        ("value_cache", C.c_void_p),
+        ("key_scale", C.c_void_p),
+        ("value_scale", C.c_void_p),
+        ("kv_block_stride", C.c_int64),
+        ("kv_head_stride", C.c_int64),
+        ("scale_block_stride", C.c_int64),
+        ("scale_head_stride", C.c_int64),
+        ("num_blocks", C.c_int64),
+        ("num_kv_heads", C.c_int32),
+        ("head_size", C.c_int32),
+        ("block_size", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares.
 _vp, _i32, _i64, _f32, _sz = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 _SQ_COMMON_TAIL = [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _vp, _sz, _vp]
@@ -144,6 +163,16 @@ SIGNATURES = {
     "pb_sample_top_p_host_settings": (C.c_int, [_vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp]),
     "pb_discontinuous_move_tokens": (
         C.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
+    "pb_fp8_fill_workspace_bytes": (_sz, [_i64, _i64, _i32]),
+    "pb_fp8_reshape_and_cache": (C.c_int, [C.POINTER(PbFp8Cache), _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _sz, _vp]),
+    "pb_fp8_gather_cached_kv": (C.c_int, [C.POINTER(PbFp8Cache), _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp]),
+    "pb_fp8_attn_plan": (C.c_int, [C.POINTER(PbAttnParams), C.POINTER(PbFp8Cache), _vp]),
+    "pb_fp8_attention_planned": (C.c_int, [C.POINTER(PbAttnParams), C.POINTER(PbFp8Cache), _vp]),
+    "pb_fp8_attention": (C.c_int, [C.POINTER(PbAttnParams), C.POINTER(PbFp8Cache), _vp]),
+    "pb_block_tables_workspace_bytes": (_sz, [_i32]),
+    "pb_build_block_tables": (
+        C.c_int, [_vp, _vp, _i32, _vp, _i32, _i64, _vp, _i32, _vp, _vp, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                  _vp, _sz, _vp]),
 }
 
 _lib = None

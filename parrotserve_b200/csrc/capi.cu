@@ -27,6 +27,20 @@ int sm_count() {
   return cached[dev];
 }
 
+int check_fp8_cache(const pb_fp8_cache* c) {
+  if (!c->key_cache || !c->value_cache || !c->key_scale || !c->value_scale) return PB_ERR_INVALID_ARG;
+  if (c->num_blocks <= 0 || c->num_kv_heads <= 0 || c->head_size <= 0 || c->block_size <= 0) return PB_ERR_INVALID_ARG;
+  if (c->block_size != 16 && c->block_size != 32) return PB_ERR_UNSUPPORTED;
+  if (c->head_size != 64 && c->head_size != 80 && c->head_size != 96 && c->head_size != 112 && c->head_size != 128 && c->head_size != 256)
+    return PB_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(c->key_cache) & 15u) || (reinterpret_cast<uintptr_t>(c->value_cache) & 15u)) return PB_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(c->key_scale) & 3u) || (reinterpret_cast<uintptr_t>(c->value_scale) & 3u)) return PB_ERR_INVALID_ARG;
+  if (c->kv_block_stride % 16 || c->kv_head_stride % 16 || c->kv_block_stride < 0) return PB_ERR_INVALID_ARG;
+  if (c->kv_head_stride < (int64_t)c->head_size * c->block_size) return PB_ERR_INVALID_ARG;
+  if (c->scale_block_stride < 0 || c->scale_head_stride < 0) return PB_ERR_INVALID_ARG;
+  return PB_OK;
+}
+
 namespace {
 
 // Events a caller asked to have recorded around the next single-query kernel launch of this thread
@@ -228,6 +242,8 @@ int validate_and_bind(const pb_attn_params* p, WsLayout* L, AttnDev* d) {
   d->slot_mapping = p->slot_mapping; d->slot_is_i64 = p->slot_is_i64;
   d->key_new = nullptr; d->value_new = nullptr;
   d->key_new_stride = p->key_new_stride; d->value_new_stride = p->value_new_stride;
+  d->key_scale = d->value_scale = nullptr;
+  d->scale_block_stride = d->scale_head_stride = 0;
   return PB_OK;
 }
 
@@ -277,6 +293,46 @@ int run_stages(const pb_attn_params* p, const AttnDev& d_in, cudaStream_t s) {
   e = launch_merge(d, p->dtype, p->head_size, s);
   if (e != cudaSuccess) return fail_launch(e);
   return PB_OK;
+}
+
+// ---- the same over the 8-bit cache ----
+// Checks, and the problem as the kernels see it: `p` with the cache in the place of its own (strides in bytes).
+int validate_and_bind_fp8(const pb_attn_params* p, const pb_fp8_cache* c, WsLayout* L, AttnDev* d) {
+  if (!p || !c) return PB_ERR_INVALID_ARG;
+  if (p->slot_mapping || p->key_new || p->value_new) return PB_ERR_INVALID_ARG;
+  if (p->head_size != c->head_size || p->block_size != c->block_size || p->num_kv_heads != c->num_kv_heads) return PB_ERR_INVALID_ARG;
+  const int rc_cache = check_fp8_cache(c);
+  if (rc_cache != PB_OK) return rc_cache;
+  if (!p->head_mapping && p->num_heads > p->num_kv_heads) return PB_ERR_INVALID_ARG;
+  pb_attn_params q = *p;
+  q.key_cache = c->key_cache; q.value_cache = c->value_cache;
+  q.kv_block_stride = c->kv_block_stride; q.kv_head_stride = c->kv_head_stride;
+  q.num_blocks = c->num_blocks;
+  const int rc = validate_and_bind(&q, L, d);
+  if (rc != PB_OK || p->num_rows == 0) return rc;
+  d->key_scale = c->key_scale; d->value_scale = c->value_scale;
+  d->scale_block_stride = c->scale_block_stride; d->scale_head_stride = c->scale_head_stride;
+  return PB_OK;
+}
+
+int run_plan_fp8(const pb_attn_params* p, const AttnDev& d, cudaStream_t s) {
+  const cudaError_t e = launch_plan(d, p->block_size, false, s);
+  return e == cudaSuccess ? PB_OK : fail_launch(e);
+}
+
+int run_stages_fp8(const pb_attn_params* p, const AttnDev& d_in, cudaStream_t s) {
+  AttnDev d = d_in;
+  d.sq_waits_at_start = 1;
+  const cudaEvent_t ev0 = g_ev_begin, ev1 = g_ev_end;
+  g_ev_begin = g_ev_end = nullptr;
+  if (ev0) cudaEventRecord(ev0, s);
+  cudaError_t e = p->dtype == PB_F16    ? launch_single_query_fp8_f16(d, p->head_size, p->block_size, s)
+                  : p->dtype == PB_BF16 ? launch_single_query_fp8_bf16(d, p->head_size, p->block_size, s)
+                                        : launch_single_query_fp8_f32(d, p->head_size, p->block_size, s);
+  if (e != cudaSuccess) return fail_launch(e);
+  if (ev1) cudaEventRecord(ev1, s);
+  e = launch_merge(d, p->dtype, p->head_size, s);
+  return e == cudaSuccess ? PB_OK : fail_launch(e);
 }
 
 int single_query_entry(void* out, const void* query, const void* key_cache, const void* value_cache,
@@ -346,6 +402,33 @@ int pb_shared_prefix_attention(const pb_attn_params* p, void* stream) {
   rc = pb::run_plan(p, d, s);
   if (rc != PB_OK) return rc;
   return pb::run_stages(p, d, s);
+}
+
+int pb_fp8_attn_plan(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream) {
+  pb::WsLayout L;
+  pb::AttnDev d;
+  const int rc = pb::validate_and_bind_fp8(p, cache, &L, &d);
+  if (rc != PB_OK || p->num_rows == 0) return rc;
+  return pb::run_plan_fp8(p, d, static_cast<cudaStream_t>(stream));
+}
+
+int pb_fp8_attention_planned(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream) {
+  pb::WsLayout L;
+  pb::AttnDev d;
+  const int rc = pb::validate_and_bind_fp8(p, cache, &L, &d);
+  if (rc != PB_OK || p->num_rows == 0) return rc;
+  return pb::run_stages_fp8(p, d, static_cast<cudaStream_t>(stream));
+}
+
+int pb_fp8_attention(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream) {
+  pb::WsLayout L;
+  pb::AttnDev d;
+  int rc = pb::validate_and_bind_fp8(p, cache, &L, &d);
+  if (rc != PB_OK || p->num_rows == 0) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = pb::run_plan_fp8(p, d, s);
+  if (rc != PB_OK) return rc;
+  return pb::run_stages_fp8(p, d, s);
 }
 
 int pb_attention_step_host(const pb_attn_params* p, const pb_host_step* io, void* stream) {

@@ -315,6 +315,10 @@ struct AttnDev {            // what the attention kernels read
   int32_t gqa_heads;          // query heads of one kv head that the 16-bit single-query kernel takes in one item (1: no sharing)
   int32_t out_vec16;          // 1: output rows may be written with 16-byte stores (base and row stride aligned)
   int64_t q_stride, out_stride, kv_block_stride, kv_head_stride, num_blocks;
+  // 8-bit cache: the scale of a (block, kv head) of K and of V; NULL for the other types
+  const float* key_scale;
+  const float* value_scale;
+  int64_t scale_block_stride, scale_head_stride;
 };
 
 // Index of the partial of (row, part, head) in the ml / acc arrays. Rows are innermost so the 128
@@ -388,6 +392,9 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
   return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
 
+// Checks of an 8-bit cache's description that every entry point over it makes. Returns a pb_status.
+int check_fp8_cache(const pb_fp8_cache* c);
+
 // SMs of the current device (queried once per device); 148 when no device can be asked.
 int sm_count();
 
@@ -396,6 +403,9 @@ cudaError_t launch_plan(const AttnDev& d, int block_size, bool dense_supported, 
 cudaError_t launch_single_query(const AttnDev& d, int dtype, int head_size, int block_size, cudaStream_t s);
 cudaError_t launch_single_query_b8(const AttnDev& d, int dtype, int head_size, cudaStream_t s);
 cudaError_t launch_single_query_b32(const AttnDev& d, int dtype, int head_size, cudaStream_t s);
+cudaError_t launch_single_query_fp8_f16(const AttnDev& d, int head_size, int block_size, cudaStream_t s);  // 8-bit cache
+cudaError_t launch_single_query_fp8_bf16(const AttnDev& d, int head_size, int block_size, cudaStream_t s);
+cudaError_t launch_single_query_fp8_f32(const AttnDev& d, int head_size, int block_size, cudaStream_t s);
 cudaError_t launch_merge(const AttnDev& d, int dtype, int head_size, cudaStream_t s);
 // Dense prefix stage; `supported` reports whether this (dtype, head, block) has a tensor-core path.
 bool dense_prefix_supported(int dtype, int head_size, int block_size);

@@ -1,0 +1,40 @@
+// Conversions of the 8-bit cache: e4m3 codes with a power-of-two (or any other) fp32 scale per (block, head).
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace pb {
+namespace fp8 {
+
+constexpr float kMax = 448.f;
+
+// Two codes (the low 16 bits of `w`) as fp16, exactly: every e4m3 value, subnormals included, is a normal fp16 value.
+__device__ __forceinline__ uint32_t to_half2(uint32_t w) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+__device__ __forceinline__ uint32_t to_half2_high(uint32_t w) { return to_half2(w >> 16); }
+__device__ __forceinline__ float2 to_float2(uint32_t w) {
+  const uint32_t h = to_half2(w);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// x * inv rounded to e4m3, to nearest even, saturating; NaN and infinities give NaN (e4m3 has no infinity).
+__device__ __forceinline__ float scaled(float x, float inv) { return fabsf(x) <= 3.402823466e38f ? __fmul_rn(x, inv) : __int_as_float(0x7fc00000); }
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return pack2(a, b) | (pack2(c, d) << 16); }
+
+// The smallest power of two s with top <= 448 * s (448 = 1.75 * 2^8), from 2^-126 on; 0 for 0. top is finite, >= 0.
+__device__ __forceinline__ float scale_for(float top) {
+  if (!(top > 0.f)) return 0.f;
+  const uint32_t bits = __float_as_uint(top);
+  const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float((uint32_t)(e < 1 ? 1 : e) << 23);
+}
+
+}  // namespace fp8
+}  // namespace pb
