@@ -316,17 +316,24 @@ int validate_and_bind_fp8(const pb_attn_params* p, const pb_fp8_cache* c, WsLayo
 }
 
 int run_plan_fp8(const pb_attn_params* p, const AttnDev& d, cudaStream_t s) {
-  const cudaError_t e = launch_plan(d, p->block_size, false, s);
+  const cudaError_t e = launch_plan(d, p->block_size, dense_prefix_supported(p->dtype, p->head_size, p->block_size), s);
   return e == cudaSuccess ? PB_OK : fail_launch(e);
 }
 
 int run_stages_fp8(const pb_attn_params* p, const AttnDev& d_in, cudaStream_t s) {
   AttnDev d = d_in;
-  d.sq_waits_at_start = 1;
+  const bool dense = (p->num_groups > 0 || p->num_segments > 0 || p->num_outer_groups > 0) &&
+                     dense_prefix_supported(p->dtype, p->head_size, p->block_size);
+  d.sq_waits_at_start = dense ? 0 : 1;
+  cudaError_t e;
+  if (dense) {
+    e = launch_dense_prefix(d, p->dtype, p->head_size, p->block_size, s);
+    if (e != cudaSuccess) return fail_launch(e);
+  }
   const cudaEvent_t ev0 = g_ev_begin, ev1 = g_ev_end;
   g_ev_begin = g_ev_end = nullptr;
   if (ev0) cudaEventRecord(ev0, s);
-  cudaError_t e = p->dtype == PB_F16    ? launch_single_query_fp8_f16(d, p->head_size, p->block_size, s)
+  e = p->dtype == PB_F16    ? launch_single_query_fp8_f16(d, p->head_size, p->block_size, s)
                   : p->dtype == PB_BF16 ? launch_single_query_fp8_bf16(d, p->head_size, p->block_size, s)
                                         : launch_single_query_fp8_f32(d, p->head_size, p->block_size, s);
   if (e != cudaSuccess) return fail_launch(e);
