@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import numpy as np
 
@@ -90,12 +91,20 @@ def context_slots(table, length, block_size):
     return np.asarray(table, dtype=np.int64)[p // block_size] * block_size + p % block_size
 
 
+class Attention(NamedTuple):
+    out: np.ndarray       # [rows, H, D]; an empty row gives zeros
+    absolute: np.ndarray  # the same weights over |V|
+    top: np.ndarray       # [rows, H] maximum of the base-2 logits
+    total: np.ndarray     # [rows, H] sum of 2^(logit - top)
+    reach: np.ndarray     # [rows, H] max over the tokens of scale * max|q| * sum |k|: what the logits of a row could be
+
+
 def attention(query, cache, contexts, scale, head_mapping=None):
     """query [rows, H, D] float64; cache = (key_codes, value_codes, key_scale, value_scale); contexts[r] = slots that row r
-    attends. Returns (out, out of the absolute values, log2-sum-exp2 maximum, sum): an empty row gives zeros."""
+    attends."""
     rows, h, d = query.shape
     out, absolute = np.zeros((rows, h, d)), np.zeros((rows, h, d))
-    top, total = np.full((rows, h), -np.inf), np.zeros((rows, h))
+    top, total, reach = np.full((rows, h), -np.inf), np.zeros((rows, h)), np.zeros((rows, h))
     mapping = list(range(h)) if head_mapping is None else list(head_mapping)
     for r in range(rows):
         if len(contexts[r]) == 0:
@@ -108,7 +117,8 @@ def attention(query, cache, contexts, scale, head_mapping=None):
             top[r, head], total[r, head] = m, p.sum()
             out[r, head] = p @ v[:, mapping[head]] / p.sum()
             absolute[r, head] = p @ np.abs(v[:, mapping[head]]) / p.sum()
-    return out, absolute, top, total
+            reach[r, head] = scale * np.abs(query[r, head]).max() * np.abs(k[:, mapping[head]]).sum(-1).max()
+    return Attention(out, absolute, top, total, reach)
 
 
 def block_tables(context_lens, new_lens, tables, free_blocks, free_head, block_size, num_tokens, num_prefills=0, prefix_lens=None):

@@ -9,17 +9,19 @@
 // partial that goes to the merge is (m, l, O * 2^(M - m)), as from every other kernel.
 //
 // Both contractions are mma.sync.m16n8k16 in fp16 with fp32 accumulation: e4m3 values are exact in fp16, so K and V are
-// converted without rounding whatever the queries' type is. Query rows of bf16 or fp32 are multiplied by the power of two
-// that puts their largest element into [2^13, 2^14) (undone in c): bf16 is then exact too (down to 2^-24 of ... 2^-38 of the
-// row's largest element), fp32 goes in as a sum of two fp16 values, whose products share the instruction (rows g and
-// g + 8 of A). w enters as hi + lo fp16 values: with one head per item both ride in one instruction as columns of B
-// (column 0 hi, column 1 lo); with several heads the columns are the heads, and lo takes an instruction of its own, which
-// only fp32 outputs get: the rounding of w alone is at most 2^-11 relative, that of a 16-bit output itself.
+// converted without rounding whatever the queries' type is. Query rows are multiplied by the power of two that puts their
+// largest element into [2^13, 2^14) (undone in c): fp16 and bf16 are then exact too (down to 2^-38 of the row's largest
+// element), fp32 goes in as a sum of two fp16 values, whose products share the instruction (rows g and g + 8 of A). w
+// enters as hi + lo fp16 values: with one head per item both ride in one instruction as columns of B (column 0 hi, column 1 lo);
+// with several heads the columns are the heads, and lo takes an instruction of its own, which only fp32 queries get: the
+// rounding of w alone is at most 2^-11 relative, that of a 16-bit output itself.
+// (mma.sync on the codes themselves is no way out: this GPU has no such instruction outside tcgen05, and its emulation
+// converts both operands in every call: 860 instructions for a (block, head) of 2 x 2 KiB, against about 400.)
 //
 // Fragments come from the tiles as they lie in the cache: a 32-bit register of ldmatrix holds four codes of one row,
-// (4t .. 4t+3) of 16, which become two fp16 pairs; the contraction index is permuted alike in both operands. The rows that
-// ldmatrix is given for K are ordered so that lane t of a quad ends with the logits of tokens 4t .. 4t+3: exactly those whose V
-// codes it holds.
+// (4t .. 4t+3) of 16, which become two fp16 pairs (the contraction index is permuted alike in both
+// operands). The rows that ldmatrix is given for K are ordered so that lane t of a quad ends with the logits of tokens
+// 4t .. 4t+3: exactly those whose V codes it holds.
 //
 // Work items, queue and copies are those of single_query.cuh: every warp streams (row, heads of one kv head, chunk of
 // blocks) items through a ring of NS stages filled by bulk copies; the scales of the blocks are read by the helper warp
@@ -126,6 +128,9 @@ template <typename T, int D, int B, int WARPS, int NS, bool MULTI>
 __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const AttnDev d) {
   using C = Sq8Cfg<T, D, B, MULTI>;
   constexpr bool kTwoParts = sizeof(T) == 4;  // fp32: q and w as hi + lo
+  constexpr int kQParts = kTwoParts ? 4 : 2;  // registers of q for each 16 elements
+  // w is largest at 2^kTop; the reference M is moved when that would pass 2^(kTop + kLag)
+  constexpr float kTop = 7.f, kLag = 8.f;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kWarpBytes = C::warp_bytes(NS);
@@ -293,14 +298,14 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
     // consumer state. Lane (g, t): row g of S (a query head, or with one head part g of w), columns 2t, 2t + 1 of O.
     constexpr int kSteps = D / 16;  // 16-code chunks of a K row = 16-row tiles of V
     const int g = lane >> 2, t = lane & 3;
-    uint32_t qa[kSteps][kTwoParts ? 4 : 2];
+    uint32_t qa[kSteps][kQParts];
     float oacc[kSteps][4];
     float m_run = -INFINITY, l_run = 0.f, ref = -INFINITY, mul = 0.f;  // m, l, M, c / (power of two of the row)
 #pragma unroll
     for (int j = 0; j < kSteps; ++j) {
       oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < (kTwoParts ? 4 : 2); ++i) qa[j][i] = 0u;
+      for (int i = 0; i < kQParts; ++i) qa[j][i] = 0u;
     }
     // ldmatrix rows. K: matrix m = lane / 8 is (chunk m / 2, n-tile m % 2), its row i token 4 (i / 2) + i % 2 + 2 (m % 2).
     // V: matrix m is rows 8m .. 8m + 7 of 32 rows of the tile.
@@ -364,22 +369,19 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
         const int qrow = MULTI ? g : 0;
         const bool live = MULTI ? g < hpi : g < 2;
         const T* qs = reinterpret_cast<const T*>(stage + 2 * C::kTileBytes) + (live ? qrow : 0) * D + 4 * t;
-        float up = 1.f;
-        mul = d.scale_log2e;
-        if constexpr (sizeof(T) == 4 || std::is_same<T, __nv_bfloat16>::value) {
-          float top = 0.f;
+        float top = 0.f;
 #pragma unroll
-          for (int c = 0; c < kSteps; ++c) {
-            float f[4];
-            load_q4<T>(qs + c * 16, f);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))));
-          }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
-          up = __uint_as_float((uint32_t)(267 - e) << 23);
-          mul *= __uint_as_float((uint32_t)(e - 13) << 23);
+        for (int c = 0; c < kSteps; ++c) {
+          float f[4];
+          load_q4<T>(qs + c * 16, f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(f[i]));
         }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
+        const float up = __uint_as_float((uint32_t)(267 - e) << 23);
+        mul = d.scale_log2e * __uint_as_float((uint32_t)(e - 13) << 23);
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           float f[4];
@@ -416,8 +418,7 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             if (c + u < kSteps) {
-              const uint32_t a[4] = {qa[c + u][0], kTwoParts ? qa[c + u][kTwoParts ? 2 : 0] : 0u, qa[c + u][1],
-                                     kTwoParts ? qa[c + u][kTwoParts ? 3 : 0] : 0u};
+              const uint32_t a[4] = {qa[c + u][0], kTwoParts ? qa[c + u][kQParts - 2] : 0u, qa[c + u][1], kTwoParts ? qa[c + u][kQParts - 1] : 0u};
               mma_f16_16816(sa, a, fp8::to_half2(kb[2 * u]), fp8::to_half2_high(kb[2 * u]));
               mma_f16_16816(sb, a, fp8::to_half2(kb[2 * u + 1]), fp8::to_half2_high(kb[2 * u + 1]));
             }
@@ -434,7 +435,7 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
         const float m_base = m_new == -INFINITY ? 0.f : m_new;  // (nothing but logits of -inf so far)
         l_run *= fast_exp2(m_run - m_base);
         m_run = m_new;
-        const bool grow = bm + lv > ref + 8.f;  // lazy reference of the weights: rescaled on jumps of more than 2^8
+        const bool grow = bm + lv > ref + kLag;  // the reference of the weights moves on jumps of more than 2^kLag
         if (__any_sync(0xffffffffu, grow)) {
           const float alpha = grow ? fast_exp2(ref - (bm + lv)) : 1.f;
           if (grow) ref = bm + lv;
@@ -443,13 +444,13 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
           for (int j = 0; j < kSteps; ++j) { oacc[j][0] *= a0; oacc[j][1] *= a1; oacc[j][2] *= a0; oacc[j][3] *= a1; }
         }
         float w[4];
-        const float shift = lv - (ref == -INFINITY ? 0.f : ref) + 7.f;
+        const float shift = lv - (ref == -INFINITY ? 0.f : ref) + kTop;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           l_run += fast_exp2(lg[i] - m_base);
           w[i] = fast_exp2(lg[i] + shift);
         }
-        uint32_t hi0, hi1, lo0 = 0u, lo1 = 0u;
+        uint32_t hi0 = 0u, hi1 = 0u, lo0 = 0u, lo1 = 0u;
         if constexpr (MULTI && !kTwoParts) {
           hi0 = pack_half2(w[0], w[1]);
           hi1 = pack_half2(w[2], w[3]);
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
       __syncwarp();  // stage s may be overwritten from here on
       if (mt.w & 512) {  // last block of the item: the partial, re-based on the exact maximum
         const int it_row = mt.x, it_head = mt.y & 0xffff, it_part = mt.y >> 16;
-        const float fix = ref == -INFINITY ? 0.f : fast_exp2(ref - 7.f - m_run);
+        const float fix = ref == -INFINITY ? 0.f : fast_exp2(ref - kTop - m_run);
         float l = l_run;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -506,12 +507,13 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
         } else {
           const size_t slot = partial_slot(d, it_row, it_part, it_head);
           const float f0 = __shfl_sync(0xffffffffu, fix, 0);
-          if (t == 0) {
-            float* ap = d.acc + slot * D + g;
+          float* ap = d.acc + slot * D + g;
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-              ap[16 * j] = (oacc[j][0] + oacc[j][1]) * f0;
-              ap[16 * j + 8] = (oacc[j][2] + oacc[j][3]) * f0;
+          for (int j = 0; j < kSteps; ++j) {
+            const float lo = oacc[j][0] + oacc[j][1], hi = oacc[j][2] + oacc[j][3];
+            if (t == 0) {
+              ap[16 * j] = lo * f0;
+              ap[16 * j + 8] = hi * f0;
             }
           }
           if (lane == 0) d.ml[slot] = make_float2(m_run, l);
@@ -529,11 +531,12 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
   if (!d.sq_waits_at_start) pdl_wait();  // the dense prefix kernel has completed
 }
 
-// Warps that fit shared memory with NS stages each (at most 8 streaming warps).
+// Streaming warps that fit shared memory with NS stages each, at most 11 (with the helper 384 threads of up to 168 registers).
+constexpr int kMaxWarps8 = 11;
 template <typename T, int D, int B, int NS, bool MULTI>
 constexpr int sq8_warps() {
   const int w = (227 * 1024 - (int)sizeof(Queue8)) / Sq8Cfg<T, D, B, MULTI>::warp_bytes(NS);
-  return w > 8 ? 8 : w;
+  return w > kMaxWarps8 ? kMaxWarps8 : w;
 }
 
 template <typename T, int D, int B, bool MULTI>
