@@ -461,7 +461,10 @@ int pb_fp8_gather_cached_kv(const pb_fp8_cache* cache, void* key, void* value, c
  * brings them), num_kv_heads, head_size and block_size have to be the cache's, and it brings no new tokens
  * (slot_mapping, key_new and value_new are NULL: the fill is a call of its own). p->dtype is the type of query and out.
  * Lists planned by one family of entry points are not valid for the other.
+ * The workspace has pb_fp8_attn_workspace_bytes(p) bytes; head_mapping and num_kv_heads are read for it besides what
+ * pb_attn_workspace_bytes reads (a head mapping need only be NULL or not).
  */
+size_t pb_fp8_attn_workspace_bytes(const pb_attn_params* p);
 int pb_fp8_attn_plan(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream);
 int pb_fp8_attention_planned(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream);
 int pb_fp8_attention(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream);

@@ -96,6 +96,7 @@ class Attention(NamedTuple):
     absolute: np.ndarray  # the same weights over |V|
     top: np.ndarray       # [rows, H] maximum of the base-2 logits
     total: np.ndarray     # [rows, H] sum of 2^(logit - top)
+    loud: np.ndarray      # [rows, H, D] the largest weight * value scale of a token, times sum |code|, over the sum of weights
     reach: np.ndarray     # [rows, H] max over the tokens of scale * max|q| * sum |k|: what the logits of a row could be
 
 
@@ -103,7 +104,7 @@ def attention(query, cache, contexts, scale, head_mapping=None):
     """query [rows, H, D] float64; cache = (key_codes, value_codes, key_scale, value_scale); contexts[r] = slots that row r
     attends."""
     rows, h, d = query.shape
-    out, absolute = np.zeros((rows, h, d)), np.zeros((rows, h, d))
+    out, absolute, loud = np.zeros((rows, h, d)), np.zeros((rows, h, d)), np.zeros((rows, h, d))
     top, total, reach = np.full((rows, h), -np.inf), np.zeros((rows, h)), np.zeros((rows, h))
     mapping = list(range(h)) if head_mapping is None else list(head_mapping)
     for r in range(rows):
@@ -117,8 +118,12 @@ def attention(query, cache, contexts, scale, head_mapping=None):
             top[r, head], total[r, head] = m, p.sum()
             out[r, head] = p @ v[:, mapping[head]] / p.sum()
             absolute[r, head] = p @ np.abs(v[:, mapping[head]]) / p.sum()
+            blocks = np.asarray(contexts[r]) // cache[1].shape[3]
+            scales = cache[3].astype(np.float64)[blocks, mapping[head]]
+            codes = np.abs(VALUES[cache[1][blocks, mapping[head], :, np.asarray(contexts[r]) % cache[1].shape[3]]])
+            loud[r, head] = (p * scales).max() * codes.sum(0) / p.sum()
             reach[r, head] = scale * np.abs(query[r, head]).max() * np.abs(k[:, mapping[head]]).sum(-1).max()
-    return Attention(out, absolute, top, total, reach)
+    return Attention(out, absolute, top, total, loud, reach)
 
 
 def block_tables(context_lens, new_lens, tables, free_blocks, free_head, block_size, num_tokens, num_prefills=0, prefix_lens=None):

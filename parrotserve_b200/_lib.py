@@ -166,6 +166,7 @@ SIGNATURES = {
     "pb_fp8_fill_workspace_bytes": (_sz, [_i64, _i64, _i32]),
     "pb_fp8_reshape_and_cache": (C.c_int, [C.POINTER(PbFp8Cache), _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _sz, _vp]),
     "pb_fp8_gather_cached_kv": (C.c_int, [C.POINTER(PbFp8Cache), _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp]),
+    "pb_fp8_attn_workspace_bytes": (_sz, [C.POINTER(PbAttnParams)]),
     "pb_fp8_attn_plan": (C.c_int, [C.POINTER(PbAttnParams), C.POINTER(PbFp8Cache), _vp]),
     "pb_fp8_attention_planned": (C.c_int, [C.POINTER(PbAttnParams), C.POINTER(PbFp8Cache), _vp]),
     "pb_fp8_attention": (C.c_int, [C.POINTER(PbAttnParams), C.POINTER(PbFp8Cache), _vp]),

@@ -22,7 +22,7 @@ CSRC = PKG / "csrc"
 OUT = PKG / "libparrot_b200_attn.so"
 OBJ_DIR = PKG / "build"
 
-SOURCES = ["capi.cu", "plan.cu", "single_query.cu", "single_query_b8.cu", "single_query_b32.cu", "merge.cu", "kv_fill.cu", "prefix_dense.cu", "dense_pair.cu", "static_scratch.cu", "block_ops.cu", "sampler.cu", "single_query_fp8_f16.cu", "single_query_fp8_bf16.cu", "single_query_fp8_f32.cu", "fp8_cache.cu", "block_tables.cu"]
+SOURCES = ["capi.cu", "plan.cu", "single_query.cu", "single_query_b8.cu", "single_query_b32.cu", "merge.cu", "kv_fill.cu", "prefix_dense.cu", "dense_pair.cu", "static_scratch.cu", "block_ops.cu", "sampler.cu", "single_query_fp8_f16.cu", "single_query_fp8_bf16.cu", "single_query_fp8_f32.cu", "decode_fp8_tc.cu", "dense_fp8.cu", "fp8_cache.cu", "block_tables.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

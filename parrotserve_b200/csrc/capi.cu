@@ -62,7 +62,7 @@ bool sq_shape_supported(int head_size, int block_size) {
 }
 
 // Static bounds -> chunking and workspace layout. Returns a pb_status.
-int compute_layout(const pb_attn_params* p, WsLayout* L) {
+int compute_layout(const pb_attn_params* p, WsLayout* L, bool kv8 = false) {
   if (!p) return PB_ERR_INVALID_ARG;
   if (p->num_rows < 0 || p->num_heads <= 0 || p->num_kv_heads <= 0 || p->head_size <= 0 ||
       p->block_size <= 0 || p->num_groups < 0 || p->suffix_table_stride < 0 || p->group_table_stride < 0 ||
@@ -145,12 +145,28 @@ int compute_layout(const pb_attn_params* p, WsLayout* L) {
   L->off_dn = off;      off = align_up(off + (size_t)cap_dn * sizeof(DnItem), 256);
   L->off_ml = off;      off = align_up(off + (size_t)rows * L->parts * H * sizeof(float2), 256);
   L->off_acc = off;     off = align_up(off + (size_t)rows * L->parts * H * p->head_size * sizeof(float), 256);
+  L->off_qparts = L->off_qmul = off;
+  if (kv8 && p->num_groups + p->num_segments + p->num_outer_groups > 0 && dense_prefix_supported(p->dtype, p->head_size, p->block_size)) {
+    off = align_up(off + (size_t)rows * H * p->head_size * (p->dtype == PB_F16 ? 3 : 2), 256);
+    L->off_qmul = off;
+    off = align_up(off + (size_t)rows * H * sizeof(float), 256);
+  }
   L->total = off;
   return PB_OK;
 }
 
-int validate_and_bind(const pb_attn_params* p, WsLayout* L, AttnDev* d) {
-  int rc = compute_layout(p, L);
+// Grouped kv heads: the largest divisor of heads / kv heads up to 8 (the columns of the MMA), so that all
+// items of a kv head hold equally many query heads. Only a call with a head mapping shares kv heads.
+int heads_per_item(const pb_attn_params* p) {
+  int heads = 1;
+  if (p->head_mapping && p->num_kv_heads > 0 && p->num_heads % p->num_kv_heads == 0)
+    for (int n = 2; n <= 8; ++n)
+      if ((p->num_heads / p->num_kv_heads) % n == 0) heads = n;
+  return heads;
+}
+
+int validate_and_bind(const pb_attn_params* p, WsLayout* L, AttnDev* d, bool kv8 = false) {
+  int rc = compute_layout(p, L, kv8);
   if (rc != PB_OK) return rc;
   if (p->num_rows == 0) return PB_OK;
   if (!p->out || !p->query || !p->key_cache || !p->value_cache) return PB_ERR_INVALID_ARG;
@@ -201,12 +217,7 @@ int validate_and_bind(const pb_attn_params* p, WsLayout* L, AttnDev* d) {
   d->acc = reinterpret_cast<float*>(ws + L->off_acc);
   d->scale_log2e = p->scale * kLog2e;
   d->num_rows = p->num_rows; d->num_heads = p->num_heads; d->num_kv_heads = p->num_kv_heads;
-  // Grouped kv heads: the largest divisor of heads / kv heads up to 8 (the columns of the MMA), so that all
-  // items of a kv head hold equally many query heads. Only a call with a head mapping shares kv heads.
-  d->gqa_heads = 1;
-  if (p->head_mapping && p->num_heads % p->num_kv_heads == 0)
-    for (int n = 2; n <= 8; ++n)
-      if ((p->num_heads / p->num_kv_heads) % n == 0) d->gqa_heads = n;
+  d->gqa_heads = heads_per_item(p);
   d->num_groups = p->num_groups;
   d->suffix_table_stride = p->suffix_table_stride; d->group_table_stride = p->group_table_stride;
   d->parts = L->parts; d->pparts = L->pparts; d->sparts = L->sparts; d->cs = L->cs; d->cp = L->cp;
@@ -244,6 +255,8 @@ int validate_and_bind(const pb_attn_params* p, WsLayout* L, AttnDev* d) {
   d->key_new_stride = p->key_new_stride; d->value_new_stride = p->value_new_stride;
   d->key_scale = d->value_scale = nullptr;
   d->scale_block_stride = d->scale_head_stride = 0;
+  d->q_parts = ws + L->off_qparts;
+  d->q_mul = reinterpret_cast<float*>(ws + L->off_qmul);
   return PB_OK;
 }
 
@@ -296,6 +309,22 @@ int run_stages(const pb_attn_params* p, const AttnDev& d_in, cudaStream_t s) {
 }
 
 // ---- the same over the 8-bit cache ----
+// Blocks per item of the single-query kernel. On tcgen05 a tile is eight blocks and an item costs about a tile beside them, so
+// items are as long as leaves two for every CTA of the chip, if the rows are half full on average. In us, with chunks of 8 / 16 /
+// 32 / 128 blocks: 64 rows of 512 tokens, 32 heads 65 / 53 / 52 / 52; 256 of 1024 431 / 346 / 341 / 326; 128 of 1024, 32 heads over 8
+// 87 / 74 / 67 / 71; 3 of 300 9.4 / 9.9 / 11.6 / 11.6. (The mma.sync kernel keeps the rule of the 16-bit caches.)
+pb_attn_params with_fp8_chunks(const pb_attn_params* p) {
+  pb_attn_params q = *p;
+  if (q.suffix_chunk_blocks <= 0 && decode_fp8_supported(q.dtype, q.head_size, q.block_size) && q.num_heads > 0 && q.num_rows > 0) {
+    const int share = heads_per_item(&q);
+    const long long ctas = (long long)sm_count() * (share > 4 ? 2 : 3);
+    const long long blocks = (long long)q.num_rows * (q.num_heads / share) * q.suffix_table_stride / 2;
+    const int cs = pow2_floor(blocks / (2 * ctas) > 0 ? blocks / (2 * ctas) : 1);
+    q.suffix_chunk_blocks = cs < 8 ? 8 : cs > 128 ? 128 : cs;
+  }
+  return q;
+}
+
 // Checks, and the problem as the kernels see it: `p` with the cache in the place of its own (strides in bytes).
 int validate_and_bind_fp8(const pb_attn_params* p, const pb_fp8_cache* c, WsLayout* L, AttnDev* d) {
   if (!p || !c) return PB_ERR_INVALID_ARG;
@@ -304,14 +333,15 @@ int validate_and_bind_fp8(const pb_attn_params* p, const pb_fp8_cache* c, WsLayo
   const int rc_cache = check_fp8_cache(c);
   if (rc_cache != PB_OK) return rc_cache;
   if (!p->head_mapping && p->num_heads > p->num_kv_heads) return PB_ERR_INVALID_ARG;
-  pb_attn_params q = *p;
+  pb_attn_params q = with_fp8_chunks(p);
   q.key_cache = c->key_cache; q.value_cache = c->value_cache;
   q.kv_block_stride = c->kv_block_stride; q.kv_head_stride = c->kv_head_stride;
   q.num_blocks = c->num_blocks;
-  const int rc = validate_and_bind(&q, L, d);
+  const int rc = validate_and_bind(&q, L, d, true);
   if (rc != PB_OK || p->num_rows == 0) return rc;
   d->key_scale = c->key_scale; d->value_scale = c->value_scale;
   d->scale_block_stride = c->scale_block_stride; d->scale_head_stride = c->scale_head_stride;
+  if (p->dense_row_tile == 0) d->dense_row_tile = 256;  // the one dense kernel here takes lone row tiles as well as pairs
   return PB_OK;
 }
 
@@ -333,9 +363,10 @@ int run_stages_fp8(const pb_attn_params* p, const AttnDev& d_in, cudaStream_t s)
   const cudaEvent_t ev0 = g_ev_begin, ev1 = g_ev_end;
   g_ev_begin = g_ev_end = nullptr;
   if (ev0) cudaEventRecord(ev0, s);
-  e = p->dtype == PB_F16    ? launch_single_query_fp8_f16(d, p->head_size, p->block_size, s)
-                  : p->dtype == PB_BF16 ? launch_single_query_fp8_bf16(d, p->head_size, p->block_size, s)
-                                        : launch_single_query_fp8_f32(d, p->head_size, p->block_size, s);
+  e = decode_fp8_supported(p->dtype, p->head_size, p->block_size) ? launch_decode_fp8(d, p->dtype, p->head_size, s)
+      : p->dtype == PB_F16  ? launch_single_query_fp8_f16(d, p->head_size, p->block_size, s)
+      : p->dtype == PB_BF16 ? launch_single_query_fp8_bf16(d, p->head_size, p->block_size, s)
+                            : launch_single_query_fp8_f32(d, p->head_size, p->block_size, s);
   if (e != cudaSuccess) return fail_launch(e);
   if (ev1) cudaEventRecord(ev1, s);
   e = launch_merge(d, p->dtype, p->head_size, s);
@@ -409,6 +440,13 @@ int pb_shared_prefix_attention(const pb_attn_params* p, void* stream) {
   rc = pb::run_plan(p, d, s);
   if (rc != PB_OK) return rc;
   return pb::run_stages(p, d, s);
+}
+
+size_t pb_fp8_attn_workspace_bytes(const pb_attn_params* p) {
+  if (!p) return 0;
+  const pb_attn_params q = pb::with_fp8_chunks(p);
+  pb::WsLayout L;
+  return pb::compute_layout(&q, &L, true) == PB_OK ? L.total : 0;
 }
 
 int pb_fp8_attn_plan(const pb_attn_params* p, const pb_fp8_cache* cache, void* stream) {

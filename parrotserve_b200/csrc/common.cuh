@@ -97,6 +97,7 @@ constexpr int32_t kDnOuter = 2;   // the item walks an outer prefix group (outer
 
 struct WsLayout {
   size_t off_rowinfo, off_sq, off_dn, off_ml, off_acc, total;
+  size_t off_qparts, off_qmul;  // (8-bit cache)
   int32_t parts;        // partial slots per row
   int32_t pparts;       // prefix partial slots per row (first `pparts` slots)
   int32_t sparts;       // suffix partial slots per row
@@ -319,6 +320,8 @@ struct AttnDev {            // what the attention kernels read
   const float* key_scale;
   const float* value_scale;
   int64_t scale_block_stride, scale_head_stride;
+  uint8_t* q_parts;  // (dense kernel) queries as e4m3 parts [parts][heads][rows][head_size], and what undoes their scaling
+  float* q_mul;      //  [heads][rows]
 };
 
 // Index of the partial of (row, part, head) in the ml / acc arrays. Rows are innermost so the 128
@@ -406,6 +409,8 @@ cudaError_t launch_single_query_b32(const AttnDev& d, int dtype, int head_size, 
 cudaError_t launch_single_query_fp8_f16(const AttnDev& d, int head_size, int block_size, cudaStream_t s);  // 8-bit cache
 cudaError_t launch_single_query_fp8_bf16(const AttnDev& d, int head_size, int block_size, cudaStream_t s);
 cudaError_t launch_single_query_fp8_f32(const AttnDev& d, int head_size, int block_size, cudaStream_t s);
+bool decode_fp8_supported(int dtype, int head_size, int block_size);  // the same on tcgen05
+cudaError_t launch_decode_fp8(const AttnDev& d, int dtype, int head_size, cudaStream_t s);
 cudaError_t launch_merge(const AttnDev& d, int dtype, int head_size, cudaStream_t s);
 // Dense prefix stage; `supported` reports whether this (dtype, head, block) has a tensor-core path.
 bool dense_prefix_supported(int dtype, int head_size, int block_size);

@@ -5,7 +5,6 @@
 #include <cuda.h>
 
 #include "common.cuh"
-#include "fp8.cuh"
 
 namespace pb {
 namespace dense {
@@ -57,6 +56,13 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64
       ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -81,6 +87,20 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
         "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -357,207 +377,14 @@ __device__ __forceinline__ bool v_tiles(const AttnDev& d, const Segment& sg, con
   return true;
 }
 
-// ---- the 8-bit cache ----
-// The codes of a kv tile are turned into 16-bit operands on their way into the rings (exactly: every e4m3 value is one of
-// fp16 and of bf16): K in the type of Q, V in fp16, as which P is written too. The scales do not touch the operands: with
-// (ks, vs) of block b a softmax thread works with
-//     lg_t = s_t * cs[b],  cs = ks * scale * log2(e)          u_t = lg_t + lv[b],  lv = log2(vs)
-//     w_t  = 2^(u_t - M + kShift)  (P, the operand of P.V)    l   += 2^-lv[b] * sum of the block's w_t
-// with M the lazy reference of max u, so that P uses fp16's range whatever the scales are. A block with vs = 0 gets zeros
-// as V and counts with lv = kMinLv, and scales below 2^kMinLv count as that: what l loses there is below 2^-26 of it.
-constexpr float kShift = 7.f;     // w <= 2^(kTau + kShift) = 2^15
-constexpr float kMinLv = -100.f;
-constexpr int kConvWarps = 4;     // converter warps for K, and as many for V: two blocks of a tile each
-
-// What the other roles need to know of a kv tile, written by a warp that walks the tiles ahead of them (list_tiles). A ring
-// of slots, each with a full and an empty barrier. Slot t is given back when a V converter has seen tile t's V slot become free: its
-// P.V has retired then, so converters and softmax threads are through with it.
-struct TileDesc {
-  int32_t blk[kTileBlocks];
-  int32_t nb, ntok, kvh, pad;  // nb == 0: no more tiles
-  float cs[kTileBlocks], lv[kTileBlocks], inv[kTileBlocks];
-};
-template <int kSlots> struct TileRing {
-  TileDesc desc[kSlots];
-  uint64_t full[kSlots], empty[kSlots];
-  __device__ __forceinline__ void init() {  // one thread
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(smem_u32(&full[i]), 32);
-      mbar_init(smem_u32(&empty[i]), 1);
-    }
-  }
-  __device__ __forceinline__ uint32_t full_bar(uint32_t tc) { return smem_u32(&full[tc % kSlots]); }
-  __device__ __forceinline__ uint32_t empty_bar(uint32_t tc) { return smem_u32(&empty[tc % kSlots]); }
-  __device__ __forceinline__ uint32_t parity(uint32_t tc) { return (tc / kSlots) & 1; }
-};
-
-// 16 codes -> 16 elements of type T, two 16-byte vectors.
-template <typename T> struct Widen;
-template <> struct Widen<__half> {
-  static __device__ __forceinline__ uint32_t two(uint32_t w) { return fp8::to_half2(w); }
-};
-template <> struct Widen<__nv_bfloat16> {
-  static __device__ __forceinline__ uint32_t two(uint32_t w) {
-    const float2 f = fp8::to_float2(w);
-    return Pack<__nv_bfloat16>::two(f.x, f.y);
-  }
-};
-template <typename T>
-__device__ __forceinline__ void widen16(const uint4& v, uint4& lo, uint4& hi) {
-  lo = make_uint4(Widen<T>::two(v.x), Widen<T>::two(v.x >> 16), Widen<T>::two(v.y), Widen<T>::two(v.y >> 16));
-  hi = make_uint4(Widen<T>::two(v.z), Widen<T>::two(v.z >> 16), Widen<T>::two(v.w), Widen<T>::two(v.w >> 16));
-}
-
-// The roles of the 8-bit kernels in warpgroups, with the registers each keeps (setmaxnreg): two of softmax threads, one of K
-// and one of V converters, one with the producer of Q and the MMA issuers. The shares sum up to what the block is launched
-// with: 256 * 144 + 256 * 72 + 128 * 48 = 640 * 96 registers.
-constexpr int kThreads8 = 640, kRegsLaunch = 96, kRegsSoftmax = 144, kRegsConvert = 72, kRegsIssue = 48;
-static_assert(256 * kRegsSoftmax + 256 * kRegsConvert + 128 * kRegsIssue <= kThreads8 * kRegsLaunch, "register shares");
-template <int kRegs> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
-template <int kRegs> __device__ __forceinline__ void regs_fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
-
-// The warp that lists the tiles: block ids, scales and extents of every kv tile of this CTA, as far ahead as the ring allows.
-// It also asks L2 for the tiles' codes (lane j: block j, K in the lower half-warp, V in the upper).
-template <int kSlots>
-__device__ __forceinline__ void list_tiles(const AttnDev& d, SegmentWalker& walk, int lane, TileRing<kSlots>* ring, volatile int* abort_flag,
-                                           int32_t* status) {
-  Segment sg;
-  uint32_t tc = 0;
-  bool ok = true;
-  while (ok && walk.next(sg)) {
-    int kvh = d.head_mapping ? d.head_mapping[sg.head] : sg.head;
-    const bool bad_head = kvh < 0 || kvh >= d.num_kv_heads;
-    if (bad_head) {
-      atomicMax(status, kStatusBadIndex);
-      kvh = 0;
-    }
-    for (int t = sg.t0; t < sg.t1; ++t, ++tc) {
-      const DenseTileView tv = dense_tile_view(d, sg.it, t);
-      const int j = lane & 15;
-      int blk = 0;
-      float ks = 0.f, vs = 0.f;
-      if (j < tv.nb) {
-        blk = tv.table[j];
-        if (blk < 0 || blk >= d.num_blocks) {
-          atomicMax(status, kStatusBadIndex);
-          blk = 0;
-        }
-        const size_t at = (size_t)blk * d.scale_block_stride + (size_t)kvh * d.scale_head_stride;
-        ks = d.key_scale[at];
-        vs = d.value_scale[at];
-        const uint8_t* base = reinterpret_cast<const uint8_t*>(lane < 16 ? d.key_cache : d.value_cache);
-        prefetch_l2(base + (size_t)blk * d.kv_block_stride + (size_t)kvh * d.kv_head_stride, kBlkBytes / 2);
-      }
-      if (tc >= kSlots && !wait_or_abort(ring->empty_bar(tc), ring->parity(tc) ^ 1, abort_flag, status, 50)) { ok = false; break; }
-      TileDesc& e = ring->desc[tc % kSlots];
-      if (lane < kTileBlocks) {
-        const float lv = vs > 0.f ? fmaxf(__log2f(vs), kMinLv) : vs == 0.f ? kMinLv : __int_as_float(0x7fc00000);
-        e.blk[lane] = vs == 0.f ? ~blk : blk;  // (the complement: its V is zero)
-        e.cs[lane] = ks * d.scale_log2e;
-        e.lv[lane] = lv;
-        e.inv[lane] = fast_exp2(-lv);
-      }
-      if (lane == 0) { e.nb = tv.nb; e.ntok = tv.ntok; e.kvh = kvh; }
-      mbar_arrive(ring->full_bar(tc));
-    }
-  }
-  if (ok && (tc < kSlots || wait_or_abort(ring->empty_bar(tc), ring->parity(tc) ^ 1, abort_flag, status, 50))) {
-    if (lane == 0) ring->desc[tc % kSlots].nb = 0;
-    mbar_arrive(ring->full_bar(tc));
-  }
-}
-
-// Converter warp pw of kConvWarps: blocks pw and pw + 4 of every kv tile of this CTA, K (kIsV == false) or V. As soon as a
-// block is converted its registers take the codes of the next tile's, which arrive while the next slot is waited for. Every
-// thread arrives on the slot's full barrier. Operand layouts as in the 16-bit kernels:
-//   K: [16-byte d chunk][block][tok][16 B], no swizzle; a lane turns the 16 codes of (chunk, token) into two vectors
-//   V: per block [d][16 tok], 32-byte rows, 32-byte swizzle; a lane turns a row. Codes behind the item's last token become 0
-template <typename T, bool kIsV, int kSlots>
-__device__ __forceinline__ void convert_tiles(const AttnDev& d, int pw, int lane, uint8_t* slots, uint32_t full0, uint32_t empty0,
-                                              TileRing<kSlots>* ring, volatile int* abort_flag, int32_t* status) {
-  constexpr int kPer = kTileBlocks / kConvWarps;
-  const uint8_t* cache = reinterpret_cast<const uint8_t*>(kIsV ? d.value_cache : d.key_cache) + lane * 16;
-  uint4 v[kPer][4];
-  auto fetch_block = [&](const TileDesc& e, uint4 (&to)[4], int j) {
-    if (j < e.nb) {
-      const int b = e.blk[j];
-      const uint4* src = reinterpret_cast<const uint4*>(cache + (size_t)(b < 0 ? ~b : b) * d.kv_block_stride + (size_t)e.kvh * d.kv_head_stride);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) to[k] = src[k * 32];
-    }
-  };
-  if (!wait_or_abort(ring->full_bar(0), 0, abort_flag, status, 50)) return;
-#pragma unroll
-  for (int u = 0; u < kPer; ++u) fetch_block(ring->desc[0], v[u], pw + u * kConvWarps);
-  for (uint32_t tc = 0;; ++tc) {
-    const TileDesc& cur = ring->desc[tc % kSlots];
-    const int nb = cur.nb;
-    if (nb == 0) break;
-    const int s = tc & 1;
-    if (!wait_or_abort(empty0 + s * 8, ((tc >> 1) & 1) ^ 1, abort_flag, status, 50)) break;
-    if (kIsV && pw == 0 && lane == 0 && tc >= 2) mbar_arrive(ring->empty_bar(tc - 2));
-    if (!wait_or_abort(ring->full_bar(tc + 1), ring->parity(tc + 1), abort_flag, status, 50)) break;
-    const TileDesc& nxt = ring->desc[(tc + 1) % kSlots];
-    uint8_t* slot = slots + s * kRingBytes;
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const int j = pw + u * kConvWarps;
-      if (j < nb) {
-        if (kIsV) {
-          const int left = cur.blk[j] < 0 ? 0 : cur.ntok - j * kB;  // tokens of the block that count
-          uint32_t m[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int n = left - 4 * i;
-            m[i] = n <= 0 ? 0u : n >= 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int row = k * 32 + lane;  // d
-            uint4 lo, hi;
-            widen16<__half>(make_uint4(v[u][k].x & m[0], v[u][k].y & m[1], v[u][k].z & m[2], v[u][k].w & m[3]), lo, hi);
-            uint8_t* p = slot + j * kBlkBytes + row * 32;
-            const int flip = ((row >> 2) & 1) << 4;  // 32-byte swizzle: the halves swap in rows 4..7 of every 8
-            *reinterpret_cast<uint4*>(p + flip) = lo;
-            *reinterpret_cast<uint4*>(p + (flip ^ 16)) = hi;
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int chunk = 2 * k + (lane >> 4);  // 16 codes of token lane % 16
-            uint4 lo, hi;
-            widen16<T>(v[u][k], lo, hi);
-            uint8_t* p = slot + (2 * chunk) * (kTileBlocks * 256) + j * 256 + (lane & 15) * 16;
-            *reinterpret_cast<uint4*>(p) = lo;
-            *reinterpret_cast<uint4*>(p + kTileBlocks * 256) = hi;
-          }
-        }
-      }
-      fetch_block(nxt, v[u], j);
-    }
-    fence_proxy_async_smem();
-    mbar_arrive(full0 + s * 8);
-  }
-}
-
-// The register shares of the 8-bit kernels only add up if the block is launched with kRegsLaunch registers a thread: a
-// build in which it is not must not run (the warps that ask for more would wait for good). Asked once per kernel.
-template <auto kKernel> cudaError_t check_register_shares() {
-  static const cudaError_t verdict = [] {
-    cudaFuncAttributes a;
-    const cudaError_t e = cudaFuncGetAttributes(&a, reinterpret_cast<const void*>(kKernel));
-    if (e != cudaSuccess) return e;
-    return a.numRegs == kRegsLaunch ? cudaSuccess : cudaErrorInvalidConfiguration;
-  }();
-  return verdict;
-}
-
 }  // namespace dense
+
+// The pair kernel over the 8-bit cache (dense_fp8.cu): query parts first, then the kernel. `pmap` is the map of the parts.
+cudaError_t launch_dense_fp8(const AttnDev& d, int dtype, const CUtensorMap& pmap, const CUtensorMap& amap, const CUtensorMap& omap,
+                             cudaStream_t s);
 
 // Row-tile-pair kernel (dense_pair.cu); the tensor maps are those launch_dense_prefix builds.
 cudaError_t launch_dense_pair(const AttnDev& d, int dtype, const CUtensorMap& vmap, const CUtensorMap& qmap,
                               const CUtensorMap& amap, const CUtensorMap& omap, cudaStream_t s);
-cudaError_t launch_dense_pair_fp8(const AttnDev& d, int dtype, const CUtensorMap& qmap, const CUtensorMap& amap,
-                                  const CUtensorMap& omap, cudaStream_t s);
 
 }  // namespace pb

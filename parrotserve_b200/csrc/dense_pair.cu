@@ -39,12 +39,8 @@ constexpr int kOffV = kOffK + kStages * kRingBytes;
 constexpr int kOffStage = kOffV + kStages * kRingBytes;
 constexpr int kOffBars = kOffStage + 2 * kStageBytes;
 constexpr int kSmemBytes = kOffBars + 512;
-using Ring8 = TileRing<8>;                               // (8-bit cache) what is known of the tiles under work
-constexpr int kSmemBytes8 = kSmemBytes + (int)sizeof(Ring8);
-static_assert(kSmemBytes8 <= 227 * 1024, "shared memory budget");
-// 8 softmax warps, K producer, V/Q producer, 2 MMA issuers; 8-bit cache: 8 softmax warps, warps 8-11, 12-15: K and V
-// converters, warp 16: Q, warps 17, 18: MMA issuers, warp 19: lists the tiles
-constexpr int threads_of(bool kv8) { return kv8 ? kThreads8 : 384; }
+static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+constexpr int kThreads = 384;                           // 8 softmax warps, K producer, V/Q producer, 2 MMA issuers
 constexpr uint32_t kTmemCols = 512;
 constexpr int kGroupThreads = 128;                       // softmax threads of one row tile
 
@@ -61,20 +57,6 @@ enum {
   kNumBars = 24
 };
 
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
-}
 
 // Maximum of 32 scores; kMasked: only the first `nvalid` columns count.
 template <bool kMasked>
@@ -161,88 +143,8 @@ __device__ __forceinline__ float row_exp128(uint32_t tmem_s, int vis, float scal
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// The same over the 8-bit cache: factor, offset and 2^-offset of the tile's blocks (convert_tiles in dense_common.cuh) take the
-// place of the one scale, and the row maximum is that of the logits with their offsets; `top` is that of the logits alone.
-template <bool kMasked>
-__device__ __forceinline__ float row_max128_8(uint32_t tmem_s, int vis, const TileDesc& e, float& top) {
-  uint32_t a[32], b[32];
-  float mx = -INFINITY;
-  auto two_blocks = [&](const uint32_t* v, int c) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float m0 = -INFINITY, m1 = -INFINITY;
-      if (!kMasked) {
-#pragma unroll
-        for (int i = 16 * h; i < 16 * h + 16; i += 4) {
-          m0 = max3(m0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-          m1 = max3(m1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-        }
-      } else {
-#pragma unroll
-        for (int i = 16 * h; i < 16 * h + 16; i += 2) {
-          m0 = fmaxf(m0, 32 * c + i < vis ? __uint_as_float(v[i]) : -INFINITY);
-          m1 = fmaxf(m1, 32 * c + i + 1 < vis ? __uint_as_float(v[i + 1]) : -INFINITY);
-        }
-      }
-      const float lg = fmaxf(m0, m1) * e.cs[2 * c + h];  // (no visible column: -inf, or NaN, which the maxima drop)
-      top = fmaxf(top, lg);
-      mx = fmaxf(mx, lg + e.lv[2 * c + h]);
-    }
-  };
-  tmem_ld32(tmem_s, a);
-#pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    tmem_wait_ld();
-    tmem_ld32(tmem_s + 32 * (c + 1), b);
-    two_blocks(a, c);
-    tmem_wait_ld();
-    if (c == 0) tmem_ld32(tmem_s + 64, a);
-    two_blocks(b, c + 1);
-  }
-  return mx;
-}
-template <bool kMasked>
-__device__ __forceinline__ float row_exp128_8(uint32_t tmem_s, int vis, const TileDesc& e, float m) {
-  uint32_t a[32], b[32], pk[16];
-  float sum = 0.f;
-  auto two_blocks = [&](const uint32_t* v, int c) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float cs = e.cs[2 * c + h], add = e.lv[2 * c + h] - m + kShift;
-      float part[2] = {0.f, 0.f};
-#pragma unroll
-      for (int i = 16 * h; i < 16 * h + 16; i += 2) {
-        float e0 = __uint_as_float(v[i]), e1 = __uint_as_float(v[i + 1]);
-        fma_pair(e0, e1, cs, add);
-        e0 = fast_exp2(e0);
-        e1 = fast_exp2(e1);
-        if (kMasked) {
-          e0 = (32 * c + i < vis) ? e0 : 0.f;
-          e1 = (32 * c + i + 1 < vis) ? e1 : 0.f;
-        }
-        part[(i >> 1) & 1] += e0 + e1;
-        pk[i >> 1] = Pack<__half>::two(e0, e1);
-      }
-      sum = fmaf(part[0] + part[1], e.inv[2 * c + h], sum);
-    }
-    tmem_st16(tmem_s + 16 * c, pk);
-  };
-  tmem_ld32(tmem_s, a);
-#pragma unroll 1
-  for (int c = 0; c < 4; c += 2) {
-    tmem_wait_ld();
-    tmem_ld32(tmem_s + 32 * (c + 1), b);
-    two_blocks(a, c);
-    tmem_wait_ld();
-    if (c == 0) tmem_ld32(tmem_s + 64, a);
-    two_blocks(b, c + 1);
-  }
-  return sum;
-}
-
-// KV8: over the 8-bit cache.
-template <typename T, bool KV8>
-__global__ void __launch_bounds__(threads_of(KV8), 1)
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
 dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
                   const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap omap) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -257,14 +159,12 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
   int32_t* status = &d.hdr[kHdrStatus];
   const uint32_t bars0 = smem_u32(bars);
   auto bar = [&](int i) { return bars0 + i * 8; };
-  constexpr int kQWarp = KV8 ? 16 : 9, kMmaWarp = KV8 ? 17 : 10;  // (the second issuer behind the first)
-  Ring8* tiles = reinterpret_cast<Ring8*>(smem + kSmemBytes);     // (KV8)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar(kBarFullK + s), KV8 ? 32 * kConvWarps : 32);  // every thread of the K producer warps arrives
+      mbar_init(bar(kBarFullK + s), 32);  // every thread of the K producer warp arrives
       mbar_init(bar(kBarEmptyK + s), 2);  // one release per MMA issuer
-      mbar_init(bar(kBarFullV + s), KV8 ? 32 * kConvWarps : 1);
+      mbar_init(bar(kBarFullV + s), 1);
       mbar_init(bar(kBarEmptyV + s), 2);
     }
     for (int x = 0; x < 2; ++x) {
@@ -277,12 +177,11 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
       mbar_init(bar(kBarTurn + x), 1);
       mbar_init(bar(kBarGroup + x), kGroupThreads);
     }
-    if constexpr (KV8) tiles->init();
     *abort_flag = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
   }
-  if (warp == kMmaWarp + 1) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+  if (warp == 11) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -297,17 +196,9 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
   SegmentWalker walk(d, blockIdx.x, min(dense_ctas_of(d), (int)gridDim.x));
   Segment sg;
 
-  if (KV8 && warp >= 8 && warp < 8 + 2 * kConvWarps) {
-    regs_fewer<kRegsConvert>();
-    if (warp < 8 + kConvWarps)
-      convert_tiles<T, false>(d, warp - 8, lane, smem + kOffK, bar(kBarFullK), bar(kBarEmptyK), tiles, abort_flag, status);
-    else
-      convert_tiles<T, true>(d, warp - 8 - kConvWarps, lane, smem + kOffV, bar(kBarFullV), bar(kBarEmptyV), tiles, abort_flag, status);
-  } else if (!KV8 && warp == 8) {
+  if (warp == 8) {
     k_producer<1>(d, walk, 0, lane, sK0, bars0, abort_flag, status);
-  } else if (warp >= kQWarp) {
-  if constexpr (KV8) regs_fewer<kRegsIssue>();  // (one place for the whole warpgroup)
-  if (warp == kQWarp) {
+  } else if (warp == 9) {
     // ============ V producer; also the Q operands of every segment ============
     // Q_x: [2 halves of d][128 rows][128 B], 128-byte swizzle, as eight boxes of 32 rows x 64
     // elements. Rows beyond the batch read as zero; rows beyond the item are other queries whose
@@ -330,7 +221,7 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
         ++segx[x];
         __syncwarp();
       }
-      if (!KV8 && ok) ok = v_tiles(d, sg, &vmap, lane, sV0, bars0, tc, abort_flag, status);
+      if (ok) ok = v_tiles(d, sg, &vmap, lane, sV0, bars0, tc, abort_flag, status);
     }
     if (!ok) {
       // drain: give copies already issued a bounded chance to land before shared memory goes away
@@ -339,7 +230,7 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
       for (int x = 0; x < 2; ++x)
         if (segx[x] > 0) (void)mbar_wait_bounded(bar(kBarQ + x), (segx[x] - 1) & 1);
     }
-  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+  } else if (warp == 10 || warp == 11) {
     // ======================= MMA issuer of row tile x =======================
     // A straight chain per kv tile i of a segment:
     //   P_x.V(i)       once P_x(i) is written and V(i) has landed (i = 0: the last epilogue has drained O_x)
@@ -358,8 +249,8 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
     //   K:   [16-byte d chunk][blk][tok][16 B], no swizzle   -> SBO 128 (8-token groups), LBO 2048 (d chunks)
     //   V:   per block [d][16 tok], 32-byte rows, 32-byte swizzle -> SBO 256 (8-row groups)
     //   P_x: tensor memory, lane = row, tokens packed two per column -> block j = columns [8j, 8j + 8)
-    const int x = warp - kMmaWarp;
-    constexpr uint32_t kIdescPV = make_idesc(128, kD, !KV8 && Pack<T>::kBf16);
+    const int x = warp - 10;
+    constexpr uint32_t kIdescPV = make_idesc(128, kD, Pack<T>::kBf16);
     const uint64_t desc_q = smem_desc(sQ + x * kQBytes, 16, 1024, 2);
     const uint64_t desc_k0 = smem_desc(sK0, 2048, 128, 0), desc_k1 = smem_desc(sK0 + kRingBytes, 2048, 128, 0);
     const uint64_t desc_v0 = smem_desc(sV0, 16, 256, 6), desc_v1 = smem_desc(sV0 + kRingBytes, 16, 256, 6);
@@ -441,11 +332,7 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
       tcx += n;
       ++segx;
     }
-  } else if constexpr (KV8) {
-    list_tiles(d, walk, lane, tiles, abort_flag, status);
-  }
   } else {
-    if constexpr (KV8) regs_more<kRegsSoftmax>();
     // ======================= softmax + epilogue: one thread per row =======================
     const int x = warp >> 2;                      // row tile of this thread's group
     const int r = (warp & 3) * 32 + lane;         // row inside the tile = TMEM lane
@@ -486,20 +373,13 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
         tc_fence_after();
         PB_TRACE(1);
         // ---- row maximum ----
-        float mx, top = -INFINITY;
-        if constexpr (KV8) {
-          if (!wait_or_abort(tiles->full_bar(tc), tiles->parity(tc), abort_flag, status)) { ok = false; break; }
-          const TileDesc& e = tiles->desc[tc % 8];
-          mx = all_valid ? row_max128_8<false>(tmem_s, vis, e, top) : row_max128_8<true>(tmem_s, vis, e, top);
-        } else {
-          top = mx = (all_valid ? row_max128<false>(tmem_s, vis) : row_max128<true>(tmem_s, vis)) * d.scale_log2e;
-        }
+        const float mx = (all_valid ? row_max128<false>(tmem_s, vis) : row_max128<true>(tmem_s, vis)) * d.scale_log2e;
         PB_TRACE(2);
         // Lazy reference maximum: the row keeps its reference m_run until a tile exceeds it by more
         // than 2^kTau; P then holds values up to 2^kTau instead of 1, which fp16/bf16 and the fp32
         // accumulators absorb, and O in TMEM is rescaled only on those rare jumps. (m, l, O) stay
         // mutually consistent, which is all the merge needs.
-        st.m_true = fmaxf(st.m_true, top);
+        st.m_true = fmaxf(st.m_true, mx);
         const bool grow = mx > st.m_run + kTau;  // true on the first tile a row sees a token in
         const float alpha = grow ? fast_exp2(st.m_run - mx) : 1.f;
         if (t > sg.t0 && __any_sync(0xffffffffu, grow && st.l_run > 0.f)) {
@@ -520,15 +400,10 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
         st.l_run *= alpha;
         st.m_run = grow ? mx : st.m_run;
         // ---- P = 2^(s - m) into the row's P columns, and the row sum ----
-        if constexpr (KV8) {
-          const TileDesc& e = tiles->desc[tc % 8];
-          st.l_run += all_valid ? row_exp128_8<false>(tmem_s, vis, e, st.m_run) : row_exp128_8<true>(tmem_s, vis, e, st.m_run);
-        } else {
-          st.l_run += all_valid ? row_exp128<T, false>(tmem_s, vis, d.scale_log2e, st.m_run)
-                                : row_exp128<T, true>(tmem_s, vis, d.scale_log2e, st.m_run);
-        }
+        st.l_run += all_valid ? row_exp128<T, false>(tmem_s, vis, d.scale_log2e, st.m_run)
+                              : row_exp128<T, true>(tmem_s, vis, d.scale_log2e, st.m_run);
         PB_TRACE(3);
-        if (!KV8 && (tv.ntok & 15)) {
+        if (tv.ntok & 15) {
           // ragged last block: zero the V columns beyond the length so 0 * (stale bytes) stays 0
           // (both groups do it, each before its own P is announced; row d of the V tile per thread)
           if (!wait_or_abort(bar(kBarFullV + s), (tc >> 1) & 1, abort_flag, status)) { ok = false; break; }
@@ -555,7 +430,7 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
       const size_t slot = partial_slot(d, row_ok ? row : it.row0, dense_part_base(d, it) + sg.part, sg.head);
       // re-base the partial on the exact row maximum; a row that saw no token in this CTA's tiles
       // (causal items) leaves the empty partial (-inf, 0, 0)
-      const float fix = (st.m_true == -INFINITY) ? 0.f : fast_exp2(st.m_run - (KV8 ? kShift : 0.f) - st.m_true);
+      const float fix = (st.m_true == -INFINITY) ? 0.f : fast_exp2(st.m_run - st.m_true);
       // Finished rows: this CTA holds every kv tile of (item, head) and the rows have no other
       // partial, so O / l IS the attention output; it goes out in the model's type and the merge
       // skips these rows (same test on its side: one dense partial, no suffix, the item's flag).
@@ -640,7 +515,7 @@ dense_pair_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, con
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp + 1) {
+  if (warp == 11) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
   }
@@ -654,26 +529,21 @@ extern "C" int pb_debug_trace_read(void* dst, size_t bytes) {
 }
 #endif
 
-template <typename T, bool KV8>
-static cudaError_t launch_pair(const AttnDev& d, const CUtensorMap& vmap, const CUtensorMap& qmap, const CUtensorMap& amap,
-                               const CUtensorMap& omap, cudaStream_t s) {
-  constexpr int smem = KV8 ? kSmemBytes8 : kSmemBytes;
-  auto kfn = dense_pair_kernel<T, KV8>;
-  cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && KV8) e = check_register_shares<dense_pair_kernel<T, KV8>>();
-  if (e != cudaSuccess) return e;
-  return launch_kernel(kfn, d.num_sms, threads_of(KV8), smem, s, true, d, vmap, qmap, amap, omap);
-}
-
 cudaError_t launch_dense_pair(const AttnDev& d, int dtype, const CUtensorMap& vmap, const CUtensorMap& qmap,
                               const CUtensorMap& amap, const CUtensorMap& omap, cudaStream_t s) {
-  return dtype == PB_F16 ? launch_pair<__half, false>(d, vmap, qmap, amap, omap, s)
-                         : launch_pair<__nv_bfloat16, false>(d, vmap, qmap, amap, omap, s);
-}
-cudaError_t launch_dense_pair_fp8(const AttnDev& d, int dtype, const CUtensorMap& qmap, const CUtensorMap& amap,
-                                  const CUtensorMap& omap, cudaStream_t s) {
-  return dtype == PB_F16 ? launch_pair<__half, true>(d, qmap, qmap, amap, omap, s)  // (the map of V is never used)
-                         : launch_pair<__nv_bfloat16, true>(d, qmap, qmap, amap, omap, s);
+  cudaError_t e;
+  if (dtype == PB_F16) {
+    auto kfn = dense_pair_kernel<__half>;
+    e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    e = launch_kernel(kfn, d.num_sms, kThreads, kSmemBytes, s, true, d, vmap, qmap, amap, omap);
+  } else {
+    auto kfn = dense_pair_kernel<__nv_bfloat16>;
+    e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    e = launch_kernel(kfn, d.num_sms, kThreads, kSmemBytes, s, true, d, vmap, qmap, amap, omap);
+  }
+  return e;
 }
 
 }  // namespace pb

@@ -8,7 +8,7 @@
 namespace pb {
 namespace fp8 {
 
-constexpr float kMax = 448.f;
+constexpr float kMinLv = -100.f;  // log2 of the smallest value scale told apart from smaller ones by the tensor-core kernels
 
 // Two codes (the low 16 bits of `w`) as fp16, exactly: every e4m3 value, subnormals included, is a normal fp16 value.
 __device__ __forceinline__ uint32_t to_half2(uint32_t w) {

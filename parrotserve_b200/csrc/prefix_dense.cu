@@ -60,13 +60,9 @@ constexpr int kOffBars = kOffV + kStages * kRingBytes;
 constexpr int kOffLsum = kOffBars + 256;            // first exchange buffer (row maxima per tile, row sums per segment)
 constexpr int kOffPmax = kOffLsum + 1024;           // second exchange buffer ([2 halves][128 rows] floats each)
 constexpr int kSmemBytes = kOffPmax + 1024;
-using Ring8 = TileRing<4>;                          // (8-bit cache) what is known of the tiles under work
-constexpr int kSmemBytes8 = kSmemBytes + (int)sizeof(Ring8);
-static_assert(kSmemBytes8 <= 227 * 1024, "shared memory budget");
+static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 constexpr int kSoftmaxThreads = 256;            // warps 0-7: two column halves x four TMEM lane quarters
-// + warps 8, 9: K producers, warp 10: V producer, warp 11: MMA issuer; 8-bit cache: + warps 8-11, 12-15: K and V converters,
-// warp 16: Q, warp 17: MMA issuer, warp 18: lists the tiles
-constexpr int threads_of(bool kv8) { return kv8 ? kThreads8 : 384; }
+constexpr int kThreads = 384;                   // + warps 8, 9: K producers, warp 10: V producer, warp 11: MMA issuer
 constexpr uint32_t kTmemCols = 512;             // S0: [0,128)  S1: [128,256)  O: [256,384)
 
 enum {
@@ -77,9 +73,8 @@ enum {
   kNumBars = 17
 };
 
-// KV8: over the 8-bit cache (convert_tiles in dense_common.cuh says how its scales enter).
-template <typename T, bool KV8>
-__global__ void __launch_bounds__(threads_of(KV8), 1)
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
 dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
                     const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap omap) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -93,14 +88,12 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kOffBars + kNumBars * 8 + 8);
   int32_t* status = &d.hdr[kHdrStatus];
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  constexpr int kVWarp = KV8 ? 16 : 10, kMmaWarp = KV8 ? 17 : 11;
-  Ring8* tiles = reinterpret_cast<Ring8*>(smem + kSmemBytes);  // (KV8)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar(kBarFullK + s), KV8 ? 32 * kConvWarps : 64);  // every thread of the K producer warps arrives
+      mbar_init(bar(kBarFullK + s), 64);  // every thread of the two K producer warps arrives
       mbar_init(bar(kBarEmptyK + s), 1);
-      mbar_init(bar(kBarFullV + s), KV8 ? 32 * kConvWarps : 1);
+      mbar_init(bar(kBarFullV + s), 1);
       mbar_init(bar(kBarEmptyV + s), 1);
       mbar_init(bar(kBarS + s), 1);
       mbar_init(bar(kBarP + s), kSoftmaxThreads);
@@ -110,12 +103,11 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
     mbar_init(bar(kBarO), 1);
     mbar_init(bar(kBarX), kSoftmaxThreads);
     mbar_init(bar(kBarY), kSoftmaxThreads);
-    if constexpr (KV8) tiles->init();
     *abort_flag = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
   }
-  if (warp == kMmaWarp) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+  if (warp == 11) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -133,13 +125,7 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
   SegmentWalker walk(d, blockIdx.x, min(dense_ctas_of(d), (int)gridDim.x));
   Segment sg;
 
-  if (KV8 && warp >= 8 && warp < 8 + 2 * kConvWarps) {
-    regs_fewer<kRegsConvert>();
-    if (warp < 8 + kConvWarps)
-      convert_tiles<T, false>(d, warp - 8, lane, smem + kOffK, bar(kBarFullK), bar(kBarEmptyK), tiles, abort_flag, status);
-    else
-      convert_tiles<T, true>(d, warp - 8 - kConvWarps, lane, smem + kOffV, bar(kBarFullV), bar(kBarEmptyV), tiles, abort_flag, status);
-  } else if (!KV8 && (warp == 8 || warp == 9)) {
+  if (warp == 8 || warp == 9) {
     // ============ K producers (2 warps): per-thread 16-byte async copies with re-pack ============
     // The 256-byte row of d-chunk c of block j goes to [c][j][16 tok][16 B]: the 8-token groups of
     // ALL blocks of the tile then sit 128 bytes apart and one MMA spans the whole tile. A warp
@@ -176,10 +162,8 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
       }
     }
     cp_async_wait_all();
-  } else if (warp >= kVWarp) {
-  if constexpr (KV8) regs_fewer<kRegsIssue>();  // (one place for the whole warpgroup)
-  if (warp == kVWarp) {
-    // ============ V producer: TMA tiled loads with the 32-byte swizzle; Q ============
+  } else if (warp == 10) {
+    // ============ V producer: TMA tiled loads with the 32-byte swizzle ============
     uint32_t tc = 0, seg_idx = 0;
     bool ok = true;
     while (ok && walk.next(sg)) {
@@ -200,7 +184,6 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
       }
       ++seg_idx;
       __syncwarp();
-      if constexpr (KV8) continue;  // (K and V are the converters')
 
       // The two-slot rings hide little latency when the single-query kernel saturates HBM beside
       // this one: ask L2 for the K and V tiles of the blocks kPrefetchTiles tiles ahead (lane j:
@@ -240,16 +223,16 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
     }
     if (!ok && (tc > 0 || seg_idx > 0)) {
       // drain: give copies already issued a bounded chance to land before shared memory goes away
-      for (uint32_t c = (tc >= 2 ? tc - 2 : 0); !KV8 && c < tc; ++c)
+      for (uint32_t c = (tc >= 2 ? tc - 2 : 0); c < tc; ++c)
         (void)mbar_wait_bounded(bar(kBarFullV + (c & 1)), (c >> 1) & 1);
       if (seg_idx > 0) (void)mbar_wait_bounded(bar(kBarQ), (seg_idx - 1) & 1);
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == 11) {
     // ======================= MMA issuer =======================
     // Polls two independent conditions so neither contraction waits behind the other's inputs:
     //   K(next) landed              -> issue S(next) = Q.K^T   (at most one tile ahead of P.V)
     //   P(cur) written, V(cur) here -> issue O += P.V
-    constexpr uint32_t kIdescPV = make_idesc(128, kD, !KV8 && Pack<T>::kBf16);
+    constexpr uint32_t kIdescPV = make_idesc(128, kD, Pack<T>::kBf16);
     uint32_t tc0 = 0, seg_ctr = 0;
     bool ok = true;
     while (ok && walk.next(sg)) {
@@ -336,11 +319,7 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
       tc0 += n;
       ++seg_ctr;
     }
-  } else if constexpr (KV8) {
-    if (warp == kMmaWarp + 1) list_tiles(d, walk, lane, tiles, abort_flag, status);
-  }
   } else {
-    if constexpr (KV8) regs_more<kRegsSoftmax>();
     // ======================= softmax + epilogue =======================
     // 256 threads. Thread (r, ch): TMEM lane r = (warp & 3) * 32 + lane, column half ch = warp >> 2.
     // With at most 64 (32) query rows in the tile the rows are loaded twice (four times) into the
@@ -366,7 +345,7 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
     Segment sg_next;
     bool have = walk.next(sg);
     while (ok && have) {
-      const bool have_next = KV8 ? false : walk.next(sg_next);
+      const bool have_next = walk.next(sg_next);
       const DnItem& it = sg.it;
       const int dup_log = (it.nrows <= 32) ? 2 : (it.nrows <= 64) ? 1 : 0;
       const int rows_per = 128 >> dup_log;         // distinct query rows in the operand
@@ -394,24 +373,7 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
         tmem_wait_ld();
         // four independent chains: a single running maximum would be 64 dependent operations
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        float cs[4], lv[4];  // (KV8) factor and offset of the four blocks of this half
-        float top = -INFINITY;  // (KV8) maximum of the logits, without the offsets
-        if constexpr (KV8) {
-          if (!wait_or_abort(tiles->full_bar(tc), tiles->parity(tc), abort_flag, status)) { ok = false; break; }
-          const TileDesc& ts = tiles->desc[tc % 4];
-          const float4 c4 = *reinterpret_cast<const float4*>(ts.cs + ch * 4), l4 = *reinterpret_cast<const float4*>(ts.lv + ch * 4);
-          cs[0] = c4.x; cs[1] = c4.y; cs[2] = c4.z; cs[3] = c4.w;
-          lv[0] = l4.x; lv[1] = l4.y; lv[2] = l4.z; lv[3] = l4.w;
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (ntok >= 64 || i < ntok) mx4[i >> 4] = fmaxf(mx4[i >> 4], __uint_as_float(v[i]));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mx4[j] *= cs[j];  // (a block without a visible column: -inf, or NaN, which the maxima below drop)
-            top = fmaxf(top, mx4[j]);
-            mx4[j] += lv[j];
-          }
-        } else if (ntok >= 64) {
+        if (ntok >= 64) {
 #pragma unroll
           for (int i = 0; i < 64; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(v[i]));
         } else {
@@ -436,8 +398,8 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
         // than 2^kTau; P then holds values up to 2^kTau instead of 1, which fp16/bf16 and the fp32
         // accumulators absorb, and O in TMEM is rescaled only on those rare jumps. (m, l, O) stay
         // mutually consistent, which is all the merge needs.
-        const float m_cand = KV8 ? mx : mx * d.scale_log2e;
-        m_true = fmaxf(m_true, KV8 ? top : m_cand);  // (KV8: of this half; the halves are joined at the segment's end)
+        const float m_cand = mx * d.scale_log2e;
+        m_true = fmaxf(m_true, m_cand);
         const bool grow = m_cand > m_run + kTau;  // always true on a row's first tile (m_run = -inf)
         const float m_new = grow ? m_cand : m_run;
         const float alpha = grow ? fast_exp2(m_run - m_new) : 1.f;
@@ -464,30 +426,7 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
         // this tile's S could be produced)
         float lsum4[4] = {0.f, 0.f, 0.f, 0.f};
         uint8_t* prow = smem + kOffP + s * kPBytes + (ch * 8) * 2048 + qrow * 16;
-        if constexpr (KV8) {
-          const float4 i4 = *reinterpret_cast<const float4*>(tiles->desc[tc % 4].inv + ch * 4);
-          const float inv[4] = {i4.x, i4.y, i4.z, i4.w};
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            if ((g >> gshift) == part) {
-              float p[8], sum2[2] = {0.f, 0.f};
-              const float add = lv[g >> 1] - m_run + kShift;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float e = fast_exp2(fmaf(__uint_as_float(v[g * 8 + i]), cs[g >> 1], add));
-                p[i] = (ntok >= 64 || g * 8 + i < ntok) ? e : 0.f;
-                sum2[i & 1] += p[i];
-              }
-              lsum4[g & 3] = fmaf(sum2[0] + sum2[1], inv[g >> 1], lsum4[g & 3]);
-              uint4 w;
-              w.x = Pack<__half>::two(p[0], p[1]);
-              w.y = Pack<__half>::two(p[2], p[3]);
-              w.z = Pack<__half>::two(p[4], p[5]);
-              w.w = Pack<__half>::two(p[6], p[7]);
-              *reinterpret_cast<uint4*>(prow + g * 2048) = w;
-            }
-          }
-        } else if (ntok >= 64) {
+        if (ntok >= 64) {
           // every column of this half is visible (all tiles but an item's last and the causal ones):
           // no per-column test; the exponentials section is bound by instruction issue, not by the
           // special-function unit
@@ -530,7 +469,7 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
         }
         l_run += (lsum4[0] + lsum4[1]) + (lsum4[2] + lsum4[3]);
         PB_TRACE(4);
-        if (!KV8 && (ntok_tile & 15) && ch == 0) {
+        if ((ntok_tile & 15) && ch == 0) {
           // ragged last block: zero the V columns beyond the length so 0 * (stale bytes) stays 0
           if (!wait_or_abort(bar(kBarFullV + s), ph, abort_flag, status)) { ok = false; break; }
           const int j = ntok_tile / 16;
@@ -549,13 +488,6 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
       if (!ok) break;
       // ---- row sums of the helper threads -> the thread that owns the row ----
       float* lsh = xbuf[tc & 1];  // not the buffer of the segment's last tile
-      if constexpr (KV8) {  // the exact maximum of the row's two halves, in both threads (lanes with equal rows agree already)
-        float* msh = lsh;
-        msh[ch * 128 + r] = m_true;
-        if (!sync_x()) { ok = false; break; }
-        m_true = fmaxf(m_true, msh[(ch ^ 1) * 128 + r]);
-        if (!sync_y()) { ok = false; break; }
-      }
       if (!owner) lsh[ch * 128 + r] = l_run;
       if (!sync_x()) { ok = false; break; }
       if (owner) {
@@ -571,7 +503,7 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
       const size_t slot = partial_slot(d, it.row0 + r, dense_part_base(d, it) + sg.part, sg.head);
       // re-base the partial on the exact row maximum; a row that saw no token in this CTA's tiles
       // (causal items) leaves the empty partial (-inf, 0, 0)
-      const float fix = (m_true == -INFINITY) ? 0.f : fast_exp2(m_run - (KV8 ? kShift : 0.f) - m_true);
+      const float fix = (m_true == -INFINITY) ? 0.f : fast_exp2(m_run - m_true);
       // Finished rows: this CTA holds every kv tile of (item, head) and the rows have no other
       // partial, so O / l IS the attention output; it goes out in the model's type and the merge
       // skips these rows (same test on its side: one dense partial, no suffix, the item's flag).
@@ -660,19 +592,15 @@ dense_prefix_kernel(const AttnDev d, const __grid_constant__ CUtensorMap vmap, c
       if (!direct && r < it.nrows && ch == 0) d.ml[slot] = make_float2(m_true, l_run * fix);
       tc_fence_before();
       ++seg_ctr;
-      if constexpr (KV8) {  // (looking one segment ahead costs registers that this form does not have)
-        have = walk.next(sg);
-      } else {
-        sg = sg_next;
-        have = have_next;
-      }
+      sg = sg_next;
+      have = have_next;
     }
     if (threadIdx.x == 0) bulk_wait_all();  // stores of the last segment have left shared memory and landed
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == 11) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
   }
@@ -734,39 +662,37 @@ bool dense_prefix_supported(int dtype, int head_size, int block_size) {
   return (dtype == PB_F16 || dtype == PB_BF16) && head_size == kD && block_size == kB;
 }
 
-template <typename T, bool KV8>
-static cudaError_t launch_single(const AttnDev& d, const CUtensorMap& vmap, const CUtensorMap& qmap, const CUtensorMap& amap,
-                                 const CUtensorMap& omap, cudaStream_t s) {
-  constexpr int smem = KV8 ? kSmemBytes8 : kSmemBytes;
-  auto kfn = dense_prefix_kernel<T, KV8>;
-  cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess && KV8) e = check_register_shares<dense_prefix_kernel<T, KV8>>();
-  if (e != cudaSuccess) return e;
-  return launch_kernel(kfn, d.num_sms, threads_of(KV8), smem, s, true, d, vmap, qmap, amap, omap);
-}
-
 cudaError_t launch_dense_prefix(const AttnDev& d, int dtype, int head_size, int block_size, cudaStream_t s) {
   if (!dense_prefix_supported(dtype, head_size, block_size)) return cudaErrorInvalidValue;
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return cudaErrorNotSupported;
-  const bool kv8 = d.key_scale != nullptr;
-  const CUtensorMapDataType elem = dtype == PB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const bool kv8 = d.key_scale != nullptr;  // the 8-bit cache: its kernel reads the codes itself, and its queries as parts
   CUtensorMap vmap;
   const cuuint64_t dims[4] = {(cuuint64_t)kB, (cuuint64_t)kD, (cuuint64_t)d.num_kv_heads, (cuuint64_t)d.num_blocks};
   const cuuint64_t strides[3] = {(cuuint64_t)kB * 2, (cuuint64_t)d.kv_head_stride * 2, (cuuint64_t)d.kv_block_stride * 2};
   const cuuint32_t box[4] = {(cuuint32_t)kB, (cuuint32_t)kD, 1, 1};
-  if (!kv8 && encode_cached(enc, &vmap, elem, 4, d.value_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_32B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != CUDA_SUCCESS)
-    return cudaErrorInvalidValue;
+  const CUtensorMapDataType elem = dtype == PB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = kv8 ? CUDA_SUCCESS
+                         : encode_cached(enc, &vmap, elem, 4, d.value_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_32B,
+                                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
   // queries: [num_rows][num_heads][128] with row stride q_stride; box = 32 rows x 64 elements of one head
   CUtensorMap qmap;
   const cuuint64_t qdims[3] = {(cuuint64_t)kD, (cuuint64_t)d.num_heads, (cuuint64_t)d.num_rows};
   const cuuint64_t qstrides[2] = {(cuuint64_t)kD * 2, (cuuint64_t)d.q_stride * 2};
   const cuuint32_t qbox[3] = {64, 1, 32};
-  const CUresult rq = encode_cached(enc, &qmap, elem, 3, d.query, qdims, qstrides, qbox, CU_TENSOR_MAP_SWIZZLE_128B,
-                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  CUresult rq;
+  if (kv8) {  // parts of the queries: [parts * heads][num_rows][128] codes; box = 128 rows
+    const cuuint64_t pdims[3] = {(cuuint64_t)kD, (cuuint64_t)d.num_rows, (cuuint64_t)d.num_heads * (dtype == PB_F16 ? 3 : 2)};
+    const cuuint64_t pstrides[2] = {(cuuint64_t)kD, (cuuint64_t)kD * d.num_rows};
+    const cuuint32_t pbox[3] = {(cuuint32_t)kD, 128, 1};
+    rq = encode_cached(enc, &qmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, d.q_parts, pdims, pstrides, pbox, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  } else {
+    rq = encode_cached(enc, &qmap, elem, 3, d.query, qdims, qstrides, qbox, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  }
   if (rq != CUDA_SUCCESS) return cudaErrorInvalidValue;
-  if (kv8) vmap = qmap;  // never used: the converters read the codes themselves
   // partial accumulators: [parts * heads * rows][128] fp32; box = 128 rows x 32 floats
   AttnDev dd = d;
   CUtensorMap amap;
@@ -798,10 +724,21 @@ cudaError_t launch_dense_prefix(const AttnDev& d, int dtype, int head_size, int 
       dd.acc_tma = 0;
     }
   }
-  if (d.dense_row_tile == 256)
-    return kv8 ? launch_dense_pair_fp8(dd, dtype, qmap, amap, omap, s) : launch_dense_pair(dd, dtype, vmap, qmap, amap, omap, s);
-  if (kv8) return dtype == PB_F16 ? launch_single<__half, true>(dd, vmap, qmap, amap, omap, s) : launch_single<__nv_bfloat16, true>(dd, vmap, qmap, amap, omap, s);
-  return dtype == PB_F16 ? launch_single<__half, false>(dd, vmap, qmap, amap, omap, s) : launch_single<__nv_bfloat16, false>(dd, vmap, qmap, amap, omap, s);
+  if (kv8) return launch_dense_fp8(dd, dtype, qmap, amap, omap, s);
+  if (d.dense_row_tile == 256) return launch_dense_pair(dd, dtype, vmap, qmap, amap, omap, s);
+  cudaError_t e;
+  if (dtype == PB_F16) {
+    auto kfn = dense_prefix_kernel<__half>;
+    e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    e = launch_kernel(kfn, d.num_sms, kThreads, kSmemBytes, s, true, dd, vmap, qmap, amap, omap);
+  } else {
+    auto kfn = dense_prefix_kernel<__nv_bfloat16>;
+    e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    e = launch_kernel(kfn, d.num_sms, kThreads, kSmemBytes, s, true, dd, vmap, qmap, amap, omap);
+  }
+  return e;
 }
 
 }  // namespace pb

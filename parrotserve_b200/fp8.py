@@ -139,6 +139,21 @@ class Fp8AttentionCall(AttentionCall):
         self._cache = PbFp8Cache()
         self._cache_ref = C.byref(self._cache)
 
+    def _take_workspace(self, workspace, shared_workspace) -> None:
+        # its size depends on the number of kv heads, which the cache brings: taken when the first one is bound
+        self._workspace_args = (workspace, shared_workspace)
+        self._sized_for = None
+
+    def _size_for(self, num_kv_heads: int) -> None:
+        self.params.num_kv_heads = num_kv_heads
+        nbytes = lib().pb_fp8_attn_workspace_bytes(self._params_ref)
+        if nbytes == 0:
+            raise _lib.PbError(_lib.PB_ERR_UNSUPPORTED, "pb_fp8_attn_workspace_bytes",
+                               f"head_size={self.params.head_size} block_size={self.params.block_size} dtype={self.dtype}")
+        self._use_workspace(nbytes, *self._workspace_args)
+        self._sized_for = num_kv_heads
+        self._planned = False
+
     def _bind_fp8(self, query, out, key_cache, value_cache, key_scale, value_scale, qk_max=None, exp_sum=None,
                   stats_mode=_lib.PB_STATS_NONE):
         p = self.params
@@ -154,8 +169,10 @@ class Fp8AttentionCall(AttentionCall):
         qs, os = query.stride(), out.stride()
         if p.num_rows and (qs[2] != 1 or qs[1] != d or os[2] != 1 or os[1] != d):
             raise RuntimeError("query/out must be dense over (head, dim)")
+        if hkv != self._sized_for:
+            self._size_for(hkv)
         p.out, p.query = out.data_ptr(), query.data_ptr()
-        p.num_kv_heads, p.q_stride, p.out_stride = hkv, qs[0], os[0]
+        p.q_stride, p.out_stride = qs[0], os[0]
         p.qk_max, p.exp_sum, p.stats_mode = _ptr(qk_max), _ptr(exp_sum), stats_mode
 
     def plan(self, query, out, key_cache, value_cache, key_scale, value_scale) -> None:

@@ -242,10 +242,20 @@ class AttentionCall:
             p.dense_row_tile = dense_row_tile
         self.params = p
         self._params_ref = C.byref(p)
+        self._planned = False
+        self._q_shape = (num_rows, num_heads, head_size)
+        self._take_workspace(workspace, shared_workspace)
+
+    def _take_workspace(self, workspace: Optional[torch.Tensor], shared_workspace: bool) -> None:
+        p = self.params
         nbytes = lib().pb_attn_workspace_bytes(self._params_ref)
         if nbytes == 0:
             raise _lib.PbError(_lib.PB_ERR_UNSUPPORTED, "pb_attn_workspace_bytes",
-                               f"head_size={head_size} block_size={block_size} dtype={dtype}")
+                               f"head_size={p.head_size} block_size={p.block_size} dtype={self.dtype}")
+        self._use_workspace(nbytes, workspace, shared_workspace)
+
+    def _use_workspace(self, nbytes: int, workspace: Optional[torch.Tensor], shared_workspace: bool) -> None:
+        p, device = self.params, self.device
         self.workspace_bytes = nbytes
         # A planned call keeps its work lists in the workspace between plan() and every run(), so it owns
         # its buffer; only the one-shot wrappers (plan + run in one library call) share a kept one.
@@ -259,8 +269,6 @@ class AttentionCall:
         if have < nbytes:
             raise _lib.PbError(_lib.PB_ERR_WORKSPACE, "AttentionCall")
         p.workspace = self.workspace.data_ptr()
-        self._planned = False
-        self._q_shape = (num_rows, num_heads, head_size)
 
     def _bind(self, query, out, key_cache, value_cache, qk_max=None, exp_sum=None, stats_mode=_lib.PB_STATS_NONE):
         p = self.params

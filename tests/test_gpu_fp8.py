@@ -55,18 +55,20 @@ def rand_rows(rng, n, h, d, dtype, size=1.0):
 def check_attention(out, want, dtype, what="", more=0.0):
     """Roundings that enter, with e the half step of the output's type:
     * the output's own: e |ref|;
-    * the weights': 2^-11 of each (rounded to fp16 by the tensor-core kernel and where several heads share an item; as three e4m3
-      parts, each within 2^-4 of what is left, 2^-12), 2^-22 (hi + lo fp16) for fp32 queries;
+    * the weights': 2^-11 of each (rounded to fp16 by the prefix kernel and where several heads share an item; as four e4m3
+      parts, each within 2^-4 of what is left, 2^-16), 2^-22 (hi + lo fp16) for fp32 queries; and the smallest step of the format
+      they take with the value's scale: parts with a largest weight of at least 2^8 end at half a step of 2^-9 / 16^3, fp16
+      with one of at least 2^7 at 2^-25: 2^-30 of the largest weight (times scale) for each token (`loud`);
     * the logits': q . k is summed in fp32 in at most 32 instructions and multiplied by rounded factors: 2^-19 of the
-      largest value the sum can reach (`reach`). As e4m3 parts, 16-bit queries are off by half a step of the smallest part, 2^-10
-      where the row's largest element is at least 2^7: 2^-17 of it for each element, 2^-17 of `reach` for the logit. A
-      change x of a logit changes its weight by x;
+      largest value the sum can reach (`reach`). 16-bit queries go in as e4m3 parts of a row whose largest element is
+      at least 2^7: of the prefix kernel the last part's half step is 2^-10, 2^-17 of that element for each of the row's, 2^-17 of
+      `reach` for the logit (the single-query kernel's is 2^-22, less than the sum's own). A change x of a logit changes its weight by x;
     * both enter numerator and denominator: twice, relative to the same attention over |V|; sums of weights: 2^-20."""
     e = torch.finfo(TYPES[dtype]).eps / 2
     weights, logits = (2.0 ** -22, 2.0 ** -19) if dtype == "f32" else (2.0 ** -11, 2.0 ** -17 + 2.0 ** -19)
     out = out.detach().double().cpu().numpy()
     assert np.isfinite(out).all(), what
-    tol = e * np.abs(want.out) + (2 * weights + 2 * logits * want.reach[..., None] + 2.0 ** -20 + more) * want.absolute + 1e-30
+    tol = e * np.abs(want.out) + (2 * weights + 2 * logits * want.reach[..., None] + 2.0 ** -20 + more) * want.absolute + 2.0 ** -30 * want.loud + 1e-30
     if dtype == "f16":
         tol = tol + 2.0 ** -25  # subnormal outputs
     worst = (np.abs(out - want.out) / tol).max() if out.size else 0.0
@@ -377,7 +379,7 @@ def test_statistics_and_merging_of_two_calls(dtype):
     want = orc.attention(q.double().cpu().numpy(), cache, contexts, d ** -0.5)
     # the first call's output is rounded to the type once more on its way
     check_attention(out, want, dtype, more=torch.finfo(TYPES[dtype]).eps / 2)
-    slack = (2.0 ** -17 + 2.0 ** -19 if dtype == "f16" else 2.0 ** -19) * want.reach * 1.5  # (base-2 logits: log2(e) < 1.5)
+    slack = 2.0 ** -19 * want.reach * 1.5  # (base-2 logits: log2(e) < 1.5)
     assert (np.abs(m.double().cpu().numpy() - want.top) <= slack).all()
     assert (np.abs(l.double().cpu().numpy() - want.total) <= (2 * slack + 2.0 ** -20) * want.total).all()
 
@@ -420,7 +422,7 @@ def test_long_cache_offsets_beyond_32_bits():
     p = torch.softmax((k2.double()[:, 0] @ q.double()[0, 0]) * d ** -0.5, 0)
     v, reach = v2.double()[:, 0], d ** -0.5 * q.double().abs().max() * k2.double().abs().sum(-1).max()
     two = lambda x: x.cpu().numpy()[None, None]  # noqa: E731
-    check_attention(out, orc.Attention(two(p @ v), two(p @ v.abs()), None, None, reach.cpu().numpy()[None, None]), "f16")
+    check_attention(out, orc.Attention(two(p @ v), two(p @ v.abs()), None, None, 0.0, reach.cpu().numpy()[None, None]), "f16")
 
 
 def test_rows_of_a_wider_tensor_and_into_one():
