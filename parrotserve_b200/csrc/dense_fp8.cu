@@ -41,7 +41,7 @@ constexpr int kGroupThreads = 128;                       // softmax threads of o
 constexpr uint32_t kTmemCols = 512;                      // S_0, S_1, O_0, O_1
 // The roles in warpgroups, with the registers each keeps (setmaxnreg): two of softmax threads, the converters, the rest. The
 // shares sum up to no more than the block is launched with.
-constexpr int kRegsLaunch = 128, kRegsSoftmax = 168, kRegsConvert = 96, kRegsIssue = 72;
+constexpr int kRegsLaunch = 128, kRegsSoftmax = 160, kRegsConvert = 96, kRegsIssue = 96;
 static_assert(256 * kRegsSoftmax + 128 * kRegsConvert + 128 * kRegsIssue <= kThreads * kRegsLaunch, "register shares");
 template <int kRegs> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs> __device__ __forceinline__ void regs_fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
@@ -58,7 +58,8 @@ enum {
   kBarODrained = 18, // the epilogue of a segment has read O_x out of tensor memory
   kBarGroup = 20,    // meeting point of the 128 softmax threads of row tile x (bounded, unlike bar.sync)
   kBarTurn = 22,     // issuer x has issued P_x.V and the next Q_x.K^T of a kv tile (pair items)
-  kNumBars = 24
+  kBarHand = 24,     // (lone row tile) group 1 has left its maxima and sums, and O_1 holds all its tiles
+  kNumBars = 25
 };
 
 // What the other roles need to know of a kv tile, written by the warp that lists them. A ring of slots, each with a full
@@ -208,7 +209,7 @@ __device__ __forceinline__ void list_tiles(const AttnDev& d, SegmentWalker& walk
       if (ti == i) {
         const float lv = cur.vs > 0.f ? fmaxf(__log2f(cur.vs), kMinLv) : cur.vs == 0.f ? kMinLv : __int_as_float(0x7fc00000);
         e.blk[j] = cur.vs == 0.f ? ~cur.blk : cur.blk;  // (the complement: its V is zero)
-        e.ks[j] = cur.ks;
+        e.ks[j] = cur.ks == 0.f ? 1e-30f : cur.ks;  // (a logit of -inf times 0 would be NaN)
         e.lv[j] = lv;
         e.inv[j] = fast_exp2(-lv);
         if (j == 0) {
@@ -455,11 +456,12 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
       mbar_init(bar(kBarP + x), kGroupThreads);
       mbar_init(bar(kBarPV + x), 1);
       mbar_init(bar(kBarQ + x), 1);
-      mbar_init(bar(kBarQFree + x), 1);
+      mbar_init(bar(kBarQFree + x), x == 0 ? 2 : 1);  // (Q_0: both issuers of a lone row tile)
       mbar_init(bar(kBarODrained + x), kGroupThreads);
       mbar_init(bar(kBarTurn + x), 1);
       mbar_init(bar(kBarGroup + x), kGroupThreads);
     }
+    mbar_init(bar(kBarHand), kGroupThreads);
     tiles->init();
     *abort_flag = 0;
     mbar_fence_init();
@@ -505,27 +507,19 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
     const int x = warp - 13;
     SegmentWalker walk = segments();
     constexpr uint32_t kIdescPV = make_idesc(128, kD, false);
-    const uint64_t desc_q = smem_desc(sQ + x * kNum * kPartBytes, 16, 1024, 2);
+    const uint64_t desc_q = smem_desc(sQ + x * kNum * kPartBytes, 16, 1024, 2), desc_q0 = smem_desc(sQ, 16, 1024, 2);
     const uint64_t desc_k0 = smem_desc(sK0, 2048, 128, 0), desc_k1 = smem_desc(sK0 + kRingK, 2048, 128, 0);
     const uint64_t desc_v0 = smem_desc(sV0, 16, 256, 6), desc_v1 = smem_desc(sV0 + kRingBytes, 16, 256, 6);
     const uint32_t tmem_s = tmem_base + x * 128, tmem_o = tmem_base + 256 + x * 128;
-    uint32_t tc = 0, tcx = 0, segx = 0, turns = 0;  // turns: kv tiles of pair items so far
+    uint32_t tc = 0, tcx = 0, seg = 0, pairs = 0, turns = 0;  // turns: kv tiles of pair items so far
     bool ok = true;
     while (ok && walk.next(sg)) {
       const int n = sg.t1 - sg.t0;
       const bool pair = sg.it.nrows > 128;
-      if (x == 1 && sg.it.nrows <= 128) {
-        // a lone row tile: nothing to compute here, but every ring slot still takes this issuer's release
-        for (int i = 0; i < n && ok; ++i, ++tc) {
-          const int s = tc & 1;
-          const uint32_t ph = (tc >> 1) & 1;
-          if (!wait_or_abort(bar(kBarFullK + s), ph, abort_flag, status, 100)) { ok = false; break; }
-          if (lane == 0) mbar_arrive(bar(kBarEmptyK + s));
-          if (!wait_or_abort(bar(kBarFullV + s), ph, abort_flag, status, 100)) { ok = false; break; }
-          if (lane == 0) mbar_arrive(bar(kBarEmptyV + s));
-        }
-        continue;
-      }
+      // A lone row tile is worked on by both groups: group x takes its kv tiles x, x + 2, ... with Q_0, S_x and O_x, and group 0
+      // joins the two O in the epilogue. (By one group alone each tile waits for the one before it: S, softmax, P.V, 3.3 us.)
+      const int first = pair ? 0 : x, step = pair ? 1 : 2;
+      const uint64_t bq = pair ? desc_q : desc_q0;
       // S_x = Q_x . K(i)^T (the caller has seen K(i) land); lane 0 only
       auto qk_mmas = [&](int i) {
         const int s = (tc + i) & 1;
@@ -536,32 +530,55 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         for (int p = 0; p < kNum; ++p)
 #pragma unroll
           for (int kk = 0; kk < kD / 32; ++kk)
-            mma_f8(tmem_s, desc_q + ((p * kPartBytes + kk * 32) >> 4), bk + ((kk * 2 * 2048) >> 4), idesc, (p | kk) ? 1u : 0u);
+            mma_f8(tmem_s, bq + ((p * kPartBytes + kk * 32) >> 4), bk + ((kk * 2 * 2048) >> 4), idesc, (p | kk) ? 1u : 0u);
         mma_commit(bar(kBarS + x));
       };
       auto qk_release = [&](int i) {
         mma_commit(bar(kBarEmptyK + ((tc + i) & 1)));
-        if (i == n - 1) mma_commit(bar(kBarQFree + x));
+        if (i + step >= n) {  // this issuer's last Q.K^T of the segment
+          mma_commit(bar(kBarQFree + (pair ? x : 0)));
+          if (x == 0 && pair) mma_commit(bar(kBarQFree));  // (the other issuer does not read Q_0)
+        }
       };
-      if (!wait_or_abort(bar(kBarQ + x), segx & 1, abort_flag, status)) { ok = false; break; }
-      if (!wait_or_abort(bar(kBarFullK + (tc & 1)), (tc >> 1) & 1, abort_flag, status)) { ok = false; break; }
-      fence_proxy_async_smem();  // K was written by per-thread async copies (generic proxy)
-      tc_fence_after();
-      if (lane == 0) {
-        qk_mmas(0);
-        qk_release(0);
+      // A wait names its phase by parity alone, so nobody may be two phases away from what it waits for. Ring slots take a release
+      // of each issuer for that reason, of a tile that is the other's too, as soon as it has landed.
+      auto full_k = [&](int i) { return wait_or_abort(bar(kBarFullK + ((tc + i) & 1)), ((tc + i) >> 1) & 1, abort_flag, status); };
+      auto full_v = [&](int i) { return wait_or_abort(bar(kBarFullV + ((tc + i) & 1)), ((tc + i) >> 1) & 1, abort_flag, status); };
+      auto pass_k = [&](int i) {
+        if (!full_k(i)) return false;
+        if (lane == 0) mbar_arrive(bar(kBarEmptyK + ((tc + i) & 1)));
+        return true;
+      };
+      auto pass_v = [&](int i) {
+        if (!full_v(i)) return false;
+        if (lane == 0) mbar_arrive(bar(kBarEmptyV + ((tc + i) & 1)));
+        return true;
+      };
+      if (!wait_or_abort(bar(kBarQ + (pair ? x : 0)), (pair && x == 1 ? pairs : seg) & 1, abort_flag, status)) { ok = false; break; }
+      if (first >= n && lane == 0) mbar_arrive(bar(kBarQFree));  // (a lone row tile of one kv tile: nothing for this issuer)
+      if (first == 1 && !pass_k(0)) { ok = false; break; }
+      if (first < n) {
+        if (!full_k(first)) { ok = false; break; }
+        fence_proxy_async_smem();  // K was written by per-thread async copies (generic proxy)
+        tc_fence_after();
+        if (lane == 0) {
+          qk_mmas(first);
+          qk_release(first);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      for (int i = 0; i < n; ++i) {
+      if (first == 1 && !pass_v(0)) { ok = false; break; }
+      for (int i = first; i < n; i += step, ++tcx) {
         const uint32_t c = tc + i;
         const int s = c & 1;
-        const bool more = i + 1 < n;
-        // what arrives early first: V(i), K(i + 1), the drained O_x; then P_x(i), which the chain hangs on
-        if (!wait_or_abort(bar(kBarFullV + s), (c >> 1) & 1, abort_flag, status)) { ok = false; break; }
-        if (more && !wait_or_abort(bar(kBarFullK + (s ^ 1)), ((c + 1) >> 1) & 1, abort_flag, status)) { ok = false; break; }
-        if (i == 0 && segx > 0 && !wait_or_abort(bar(kBarODrained + x), (segx - 1) & 1, abort_flag, status)) { ok = false; break; }
+        const bool more = i + step < n;
+        // what arrives early first: V(i), the next K; then P_x(i), which the chain hangs on, and the drained O_x (behind P_x: an
+        // issuer without a tile in the last segment knows by it that the segment before that is over)
+        if (!full_v(i)) { ok = false; break; }
+        if (pair && more && !full_k(i + 1)) { ok = false; break; }
         fence_proxy_async_smem();
-        if (!wait_or_abort(bar(kBarP + x), (tcx + i) & 1, abort_flag, status)) { ok = false; break; }
+        if (!wait_or_abort(bar(kBarP + x), tcx & 1, abort_flag, status)) { ok = false; break; }
+        if (i == first && seg > 0 && !wait_or_abort(bar(kBarODrained + x), (seg - 1) & 1, abort_flag, status)) { ok = false; break; }
         if (pair && (x == 1 || turns > 0) &&
             !wait_or_abort(bar(kBarTurn + (x ^ 1)), (x == 1 ? turns : turns - 1) & 1, abort_flag, status)) { ok = false; break; }
         tc_fence_after();
@@ -570,20 +587,38 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
           const uint64_t bv = s ? desc_v1 : desc_v0;
 #pragma unroll
           for (int j = 0; j < kTileBlocks; ++j)
-            if (j < nb) mma_f16_ts(tmem_o, tmem_s + j * 8, bv + j * (kBlkBytes >> 4), kIdescPV, (i > 0 || j > 0) ? 1u : 0u);
-          if (more) qk_mmas(i + 1);  // behind P_x.V(i) in the pipe: it overwrites S_x / P_x
-          if (pair) mbar_arrive(bar(kBarTurn + x));
+            if (j < nb) mma_f16_ts(tmem_o, tmem_s + j * 8, bv + j * (kBlkBytes >> 4), kIdescPV, (i > first || j > 0) ? 1u : 0u);
+          // (before the next S is announced: a softmax thread waits for this phase only with its last tile)
           mma_commit(bar(kBarPV + x));
           mma_commit(bar(kBarEmptyV + s));
-          if (more) qk_release(i + 1);
+          if (pair) {
+            if (more) qk_mmas(i + 1);  // behind P_x.V(i) in the pipe: it overwrites S_x / P_x
+            mbar_arrive(bar(kBarTurn + x));
+            if (more) qk_release(i + 1);
+          }
         }
         if (pair) ++turns;
         __syncwarp();
+        if (!pair) {
+          // the tile behind it is the other issuer's; the K of the next one of this issuer comes into the slot of this tile
+          if (i + 1 < n && !pass_k(i + 1)) { ok = false; break; }
+          if (more) {
+            if (!full_k(i + 2)) { ok = false; break; }
+            fence_proxy_async_smem();
+            tc_fence_after();
+            if (lane == 0) {
+              qk_mmas(i + 2);
+              qk_release(i + 2);
+            }
+            __syncwarp();
+          }
+          if (i + 1 < n && !pass_v(i + 1)) { ok = false; break; }
+        }
       }
       if (!ok) break;
       tc += n;
-      tcx += n;
-      ++segx;
+      ++seg;
+      if (pair) ++pairs;
     }
   }
   } else {
@@ -597,8 +632,9 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
     const uint32_t tmem_o = tmem_base + 256 + x * 128 + lane_base;
     uint8_t* const stage = smem + L::kOffStage + x * kStageBytes;
     const bool issuer = (r == 0);                 // issues the group's TMA stores
-    uint32_t tc = 0, tcx = 0, segx = 0, group_use = 0;
+    uint32_t tc = 0, tcx = 0, seg = 0, hands = 0, group_use = 0;  // hands: lone row tiles so far
     bool ok = true, store_pending = false;
+    float* const hand = reinterpret_cast<float*>(smem + L::kOffStage + kStageBytes);  // [3][128], in group 1's staging buffer
     auto group_sync = [&]() -> bool {
       mbar_arrive(bar(kBarGroup + x));
       return wait_or_abort(bar(kBarGroup + x), (group_use++) & 1, abort_flag, status);
@@ -613,14 +649,13 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
     };
     while (ok && walk.next(sg)) {
       const DnItem& it = sg.it;
-      if (x == 1 && it.nrows <= 128) {  // a lone row tile: nothing for this group
-        tc += sg.t1 - sg.t0;
-        continue;
-      }
-      const int qrow = x * 128 + r;     // row inside the item
+      const bool pair = it.nrows > 128;
+      const int first = sg.t0 + (pair ? 0 : x), step = pair ? 1 : 2;
+      const int qrow = (pair ? x * 128 : 0) + r;  // row inside the item
       RowState st = {-INFINITY, 0.f, -INFINITY};
       const float mul = d.q_mul[(size_t)sg.head * d.num_rows + min(it.row0 + qrow, d.num_rows - 1)];
-      for (int t = sg.t0; t < sg.t1; ++t, ++tc, ++tcx) {
+      for (int t = first; t < sg.t1; t += step, ++tcx) {
+        const uint32_t tc_t = tc + (t - sg.t0);
         const DenseTileView tv = dense_tile_view(d, it, t);
         // columns this row may attend: all of the tile's tokens, or (causal tile) the first causal0 + row
         const int vis = tv.causal ? min(tv.ntok, tv.causal0 + qrow) : tv.ntok;
@@ -628,8 +663,8 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         if (!wait_or_abort(bar(kBarS + x), tcx & 1, abort_flag, status)) { ok = false; break; }
         tc_fence_after();
         // ---- row maximum ----
-        if (!wait_or_abort(tiles->full_bar(tc), tiles->parity(tc), abort_flag, status)) { ok = false; break; }
-        const TileDesc& e = tiles->desc[tc % kDescSlots];
+        if (!wait_or_abort(tiles->full_bar(tc_t), tiles->parity(tc_t), abort_flag, status)) { ok = false; break; }
+        const TileDesc& e = tiles->desc[tc_t % kDescSlots];
         float top = -INFINITY;
         const float mx = all_valid ? row_max128<false>(tmem_s, vis, e, mul, top) : row_max128<true>(tmem_s, vis, e, mul, top);
         // Lazy reference maximum: the row keeps its reference m_run until a tile exceeds it by more
@@ -639,7 +674,7 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         st.m_true = fmaxf(st.m_true, top);
         const bool grow = mx > st.m_run + kTau;  // true on the first tile a row sees a token in
         const float alpha = grow ? fast_exp2(st.m_run - mx) : 1.f;
-        if (t > sg.t0 && __any_sync(0xffffffffu, grow && st.l_run > 0.f)) {
+        if (t > first && __any_sync(0xffffffffu, grow && st.l_run > 0.f)) {
           // rescale this warp's O rows in TMEM (the previous tile's P.V, which accumulated into
           // them, retired before this tile's S was produced)
           if (!wait_or_abort(bar(kBarPV + x), (tcx - 1) & 1, abort_flag, status)) { ok = false; break; }
@@ -663,10 +698,49 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         mbar_arrive(bar(kBarP + x));
       }
       if (!ok) break;
+      tc += sg.t1 - sg.t0;
       // ---- epilogue: O_x rows -> un-normalised partials, or the finished output rows ----
-      if (!wait_or_abort(bar(kBarPV + x), (tcx - 1) & 1, abort_flag, status)) { ok = false; break; }
+      if (sg.t1 > first && !wait_or_abort(bar(kBarPV + x), (tcx - 1) & 1, abort_flag, status)) { ok = false; break; }
       tc_fence_after();
-      const int nrows_x = min(128, it.nrows - x * 128);
+      if (!pair) {
+        const bool both = sg.t1 - sg.t0 > 1;
+        if (x == 1) {
+          // hand over: O_1 stays where it is, lane for lane beside O_0. The last hand-over has been read by now.
+          if (seg > 0 && !wait_or_abort(bar(kBarODrained + 1), (seg - 1) & 1, abort_flag, status)) { ok = false; break; }
+          if (!stage_begin()) { ok = false; break; }
+          hand[r] = st.m_run;
+          hand[128 + r] = st.l_run;
+          hand[256 + r] = st.m_true;
+          tc_fence_before();
+          mbar_arrive(bar(kBarHand));
+          ++seg;
+          continue;
+        }
+        if (!wait_or_abort(bar(kBarHand), hands & 1, abort_flag, status)) { ok = false; break; }
+        ++hands;
+        tc_fence_after();
+        if (both) {
+          const float m1 = hand[r], l1 = hand[128 + r];
+          st.m_true = fmaxf(st.m_true, hand[256 + r]);
+          const float m = fmaxf(st.m_run, m1), base = m == -INFINITY ? 0.f : m;
+          const float a0 = fast_exp2(st.m_run - base), a1 = fast_exp2(m1 - base);
+          uint32_t o[32], q[32];
+#pragma unroll 1
+          for (int c0 = 0; c0 < kD; c0 += 32) {
+            tmem_ld32(tmem_o + c0, o);
+            tmem_ld32(tmem_o + 128 + c0, q);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(fmaf(__uint_as_float(q[i]), a1, __uint_as_float(o[i]) * a0));
+            tmem_st32(tmem_o + c0, o);
+          }
+          tmem_wait_st();
+          st.l_run = fmaf(l1, a1, st.l_run * a0);
+          st.m_run = m;
+        }
+      }
+      const int nrows_x = min(128, it.nrows - (pair ? x * 128 : 0));
       const bool row_ok = r < nrows_x;
       const int row = it.row0 + qrow;
       const size_t slot = partial_slot(d, row_ok ? row : it.row0, dense_part_base(d, it) + sg.part, sg.head);
@@ -748,8 +822,9 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
       }
       if (!ok) break;
       tc_fence_before();
+      if (!pair) mbar_arrive(bar(kBarODrained + 1));
       mbar_arrive(bar(kBarODrained + x));
-      ++segx;
+      ++seg;
     }
     if (issuer) bulk_wait_all();  // stores of the last segment have left shared memory and landed
   }

@@ -336,6 +336,10 @@ LAYERS = [
     dict(heads=8, kv=2, prefixes=(260,), group_rows=(52,), segments=((40, 0), (2, 33)), suffixes=(0, 1, 31, 32, 33, 200, 3, 4, 5, 6)),
     dict(heads=2, kv=2, prefixes=(48, 90), group_rows=(6, 5), suffixes=tuple([20] * 11), outer=200),
     dict(heads=2, kv=2, d=64, b=32, prefixes=(100,), group_rows=(7,), segments=((3, 10),), suffixes=(5, 40, 41, 1)),
+    # shares of the chip that begin and end inside heads: CTAs with segments of one kv tile, two, and many
+    dict(heads=5, kv=5, prefixes=(4000,), group_rows=(6,), suffixes=(1, 2, 3, 4, 5, 6)),
+    dict(heads=3, kv=3, prefixes=(1500, 3000, 130, 700), group_rows=(7, 140, 20, 5), suffixes=tuple(range(172))),
+    dict(heads=4, kv=1, segments=((300, 500), (20, 0), (140, 900), (1, 700), (260, 0)), suffixes=(30, 0)),
     dict(heads=1, kv=1, segments=((700, 0), (600, 100)), dense_row_tile=256),
     dict(heads=1, kv=1, prefixes=(300,), group_rows=(600,), segments=((250, 0), (349, 20)), suffixes=(50,), dense_row_tile=256),
 ]
