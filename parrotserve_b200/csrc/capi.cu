@@ -342,6 +342,11 @@ int validate_and_bind_fp8(const pb_attn_params* p, const pb_fp8_cache* c, WsLayo
   d->key_scale = c->key_scale; d->value_scale = c->value_scale;
   d->scale_block_stride = c->scale_block_stride; d->scale_head_stride = c->scale_head_stride;
   if (p->dense_row_tile == 0) d->dense_row_tile = 256;  // the one dense kernel here takes lone row tiles as well as pairs
+  // The dense kernel gets every SM and the single-query kernel those it has left: beside a stream of codes at full HBM bandwidth
+  // a kv tile of the dense kernel takes half as long again. (256 rows over a 4096-token prefix and 512 tokens of their own, 32 heads:
+  // 276 us with the 16-bit cache's split, 27 SMs, 222 with all; 64 rows, 272 tokens: 90 and 83; 148 of 148 SMs is at most 2%
+  // from the best share.)
+  if (p->dense_ctas == 0) d->dense_ctas = d->num_sms;
   return PB_OK;
 }
 

@@ -588,14 +588,14 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
 #pragma unroll
           for (int j = 0; j < kTileBlocks; ++j)
             if (j < nb) mma_f16_ts(tmem_o, tmem_s + j * 8, bv + j * (kBlkBytes >> 4), kIdescPV, (i > first || j > 0) ? 1u : 0u);
-          // (before the next S is announced: a softmax thread waits for this phase only with its last tile)
-          mma_commit(bar(kBarPV + x));
-          mma_commit(bar(kBarEmptyV + s));
           if (pair) {
             if (more) qk_mmas(i + 1);  // behind P_x.V(i) in the pipe: it overwrites S_x / P_x
             mbar_arrive(bar(kBarTurn + x));
-            if (more) qk_release(i + 1);
           }
+          // (before the next S is announced: a softmax thread waits for this phase only with its last tile)
+          mma_commit(bar(kBarPV + x));
+          mma_commit(bar(kBarEmptyV + s));
+          if (pair && more) qk_release(i + 1);
         }
         if (pair) ++turns;
         __syncwarp();
