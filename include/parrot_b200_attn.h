@@ -442,7 +442,8 @@ typedef struct pb_fp8_cache {
  *   leave the normal range of e4m3, as long as both scales are powers of two)
  * Tokens of a block may stand anywhere in slot_mapping; of tokens with the same slot the last in the list counts. A
  * negative slot, or one outside the cache, skips its token. Rows are fp32, fp16 or bf16 (dtype).
- * workspace: pb_fp8_fill_workspace_bytes(num_tokens, num_blocks, block_size) bytes of scratch, contents irrelevant.
+ * workspace: pb_fp8_fill_workspace_bytes(num_tokens, num_blocks, block_size) bytes of scratch, contents irrelevant; none (0) for
+ * few tokens.
  */
 size_t pb_fp8_fill_workspace_bytes(int64_t num_tokens, int64_t num_blocks, int32_t block_size);
 int pb_fp8_reshape_and_cache(const pb_fp8_cache* cache, const void* key, const void* value, const void* slot_mapping,
@@ -488,7 +489,8 @@ int pb_fp8_attention(const pb_attn_params* p, const pb_fp8_cache* cache, void* s
  * row_offsets [num_requests + 1]: first row of every request (its first num_prefills + 1 entries are seg_row_offsets);
  * kv_lens [num_requests]: tokens held afterwards (the first num_prefills entries are seg_kv_lens);
  * *free_head_out: entries of free_blocks taken so far. Only block_tables is changed in place, so the call can be repeated.
- * suffix_tables may be NULL. Negative lengths count as 0. workspace: pb_block_tables_workspace_bytes(num_requests) bytes.
+ * suffix_tables may be NULL. Negative lengths count as 0. workspace: pb_block_tables_workspace_bytes(num_requests) bytes, 0
+ * for up to a thousand requests.
  */
 size_t pb_block_tables_workspace_bytes(int32_t num_requests);
 int pb_build_block_tables(const int32_t* context_lens, const int32_t* new_lens, int32_t num_requests, int32_t* block_tables,

@@ -570,7 +570,7 @@ cudaError_t launch_rows(const Fp8Rows& a, int dtype, int block_size, bool fill, 
 extern "C" {
 
 size_t pb_fp8_fill_workspace_bytes(int64_t num_tokens, int64_t num_blocks, int32_t block_size) {
-  if (num_tokens < 0 || num_blocks < 0 || block_size <= 0 || num_blocks > (int64_t)1 << 40) return 0;
+  if (num_tokens <= pb::kScanTokens || num_blocks < 0 || block_size <= 0 || num_blocks > (int64_t)1 << 40) return 0;
   return (size_t)num_blocks * block_size * sizeof(int32_t);
 }
 
@@ -580,9 +580,8 @@ int pb_fp8_reshape_and_cache(const pb_fp8_cache* cache, const void* key, const v
   pb::Fp8Rows a;
   const int rc = pb::bind_rows(cache, key, value, slot_mapping, slot_is_i64, num_tokens, key_stride, value_stride, dtype, &a);
   if (rc != PB_OK || num_tokens == 0) return rc;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
-      workspace_bytes < pb_fp8_fill_workspace_bytes(num_tokens, cache->num_blocks, cache->block_size))
-    return PB_ERR_WORKSPACE;
+  const size_t need = pb_fp8_fill_workspace_bytes(num_tokens, cache->num_blocks, cache->block_size);
+  if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < need)) return PB_ERR_WORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
   if (num_tokens > pb::kScanTokens) {

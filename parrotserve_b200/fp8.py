@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from ._lib import PbFp8Cache, check, lib
-from .ops import _DTYPES, AttentionCall, Workspace, _dtype_code, _flat_slots, _kv_geometry, _ptr, _require_cuda, _single_group_meta, _stream
+from .ops import _DTYPES, AttentionCall, Workspace, _dtype_code, _flat_slots, _kv_geometry, _ptr, _require_cuda, _single_group_meta
 
 CACHE_DTYPE = torch.float8_e4m3fn
 _NOTHING = contextlib.nullcontext()
@@ -41,13 +41,13 @@ def fp8_kv_cache(num_blocks: int, num_kv_heads: int, head_size: int, block_size:
 
 def _describe(c: PbFp8Cache, key_cache, value_cache, key_scale, value_scale):
     """Fills `c` with the four tensors' addresses and strides; returns (num_kv_heads, head_size, block_size)."""
-    _require_cuda(key_cache, value_cache, key_scale, value_scale)
     if key_cache.dtype != CACHE_DTYPE or value_cache.dtype != CACHE_DTYPE:
         raise RuntimeError("key_cache and value_cache must be torch.float8_e4m3fn")
     nb, hkv, d, b, kbs, khs = _kv_geometry(key_cache, value_cache)
     if key_scale.dtype != torch.float32 or value_scale.dtype != torch.float32:
         raise RuntimeError("key_scale and value_scale must be float32")
-    if key_scale.shape != (nb, hkv) or value_scale.shape != (nb, hkv):
+    shape = (nb, hkv)
+    if key_scale.shape != shape or value_scale.shape != shape:
         raise RuntimeError("key_scale and value_scale must be [num_blocks, num_kv_heads]")
     ss = key_scale.stride()
     if value_scale.stride() != ss:
@@ -60,33 +60,40 @@ def _describe(c: PbFp8Cache, key_cache, value_cache, key_scale, value_scale):
     return hkv, d, b
 
 
-def _on(device: torch.device):
+def _on(index: Optional[int]):
     """Makes the tensors' device the current one for a library call (nothing to do when it is)."""
-    return _NOTHING if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+    return _NOTHING if index is None or index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
-def _same_device(first: torch.Tensor, *others) -> None:
-    for t in others:
-        if t is not None and t.device != first.device:
+def _one_device(*tensors) -> int:
+    """The index of the one GPU that all tensors are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:  # (-1: the CPU)
+            _require_cuda(*tensors)
             raise RuntimeError("all tensors of a call must be on one device")
+    return index
 
 
 def _rows(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping):
-    _require_cuda(key, value, slot_mapping)
-    _same_device(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
-    if key.shape != value.shape or key.dim() != 3:
+    index = _one_device(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
+    shape = key.shape
+    if shape != value.shape or len(shape) != 3:
         raise RuntimeError("key and value must both be [num_tokens, num_heads, head_size]")
     if key.dtype != value.dtype:
         raise RuntimeError("key and value must share a dtype")
     c = PbFp8Cache()
     hkv, d, _ = _describe(c, key_cache, value_cache, key_scale, value_scale)
-    if key.shape[1:] != (hkv, d):
+    t, h, hd = shape
+    if h != hkv or hd != d:
         raise RuntimeError("cache heads/head_size differ from key's")
-    t = key.shape[0]
-    for x in (key, value):
-        if t and (x.stride(2) != 1 or x.stride(1) != d):
-            raise RuntimeError("key/value must be dense over (head, dim)")
-    return c, t, _flat_slots(slot_mapping, t)
+    ks, vs = key.stride(), value.stride()
+    if t and (ks[2] != 1 or ks[1] != d or vs[2] != 1 or vs[1] != d):
+        raise RuntimeError("key/value must be dense over (head, dim)")
+    slots = _flat_slots(slot_mapping, t)
+    # what both entry points take behind the cache
+    return c, t, index, (slots, key.data_ptr(), value.data_ptr(), slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0, t, ks[0], vs[0],
+                         _dtype_code(key))
 
 
 def fp8_reshape_and_cache(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping) -> None:
@@ -97,28 +104,24 @@ def fp8_reshape_and_cache(key, value, key_cache, value_cache, key_scale, value_s
     tokens' largest element fits (448 codes); when it grows the tokens that the block holds already are re-quantised. A
     call that brings the token at offset 0 of a block begins the block anew: what it held, its scale included, is void. Tokens of
     a block may stand in any order; of tokens with one slot the last counts. NaN and infinities are cached as NaN."""
-    c, t, slots = _rows(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
+    c, t, index, (_slots, *args) = _rows(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
     if t == 0:
         return
-    with _on(key.device):
+    with _on(index):
         nbytes = lib().pb_fp8_fill_workspace_bytes(t, c.num_blocks, c.block_size)
-        ws = Workspace.get(key.device, nbytes)
-        rc = lib().pb_fp8_reshape_and_cache(
-            C.byref(c), key.data_ptr(), value.data_ptr(), slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0, t,
-            key.stride(0), value.stride(0), _dtype_code(key), ws.data_ptr(), ws.numel(), _stream(key))
+        ws = Workspace.get(key.device, nbytes) if nbytes else None  # (a small call needs none)
+        rc = lib().pb_fp8_reshape_and_cache(C.byref(c), *args, _ptr(ws), nbytes, torch._C._cuda_getCurrentRawStream(index))
     check(rc, "pb_fp8_reshape_and_cache")
 
 
 def fp8_gather_cached_kv(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping) -> None:
     """Rows out of the cache: ``key[t], value[t]`` = code * scale of slot ``slot_mapping[t]``, rounded once to the rows' type.
     Rows with a negative slot stay as they were."""
-    c, t, slots = _rows(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
+    c, t, index, (_slots, *args) = _rows(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
     if t == 0:
         return
-    with _on(key.device):
-        rc = lib().pb_fp8_gather_cached_kv(
-            C.byref(c), key.data_ptr(), value.data_ptr(), slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0, t,
-            key.stride(0), value.stride(0), _dtype_code(key), _stream(key))
+    with _on(index):
+        rc = lib().pb_fp8_gather_cached_kv(C.byref(c), *args, torch._C._cuda_getCurrentRawStream(index))
     check(rc, "pb_fp8_gather_cached_kv")
 
 
@@ -134,7 +137,7 @@ class Fp8AttentionCall(AttentionCall):
             raise RuntimeError(f"unsupported dtype {kwargs['dtype']}")
         if kwargs["block_size"] not in (16, 32):
             raise _lib.PbError(_lib.PB_ERR_UNSUPPORTED, "Fp8AttentionCall", f"block_size={kwargs['block_size']}")
-        with _on(torch.device(kwargs["device"])):
+        with _on(torch.device(kwargs["device"]).index):
             super().__init__(**kwargs)
         self._cache = PbFp8Cache()
         self._cache_ref = C.byref(self._cache)
@@ -157,8 +160,7 @@ class Fp8AttentionCall(AttentionCall):
     def _bind_fp8(self, query, out, key_cache, value_cache, key_scale, value_scale, qk_max=None, exp_sum=None,
                   stats_mode=_lib.PB_STATS_NONE):
         p = self.params
-        _require_cuda(query, out)
-        _same_device(query, out, key_cache, value_cache, key_scale, value_scale)
+        index = _one_device(query, out, key_cache, value_cache, key_scale, value_scale)
         hkv, d, b = _describe(self._cache, key_cache, value_cache, key_scale, value_scale)
         if query.dtype != self.dtype or out.dtype != self.dtype:
             raise RuntimeError("query and out must have the dtype of the call")
@@ -174,21 +176,22 @@ class Fp8AttentionCall(AttentionCall):
         p.out, p.query = out.data_ptr(), query.data_ptr()
         p.q_stride, p.out_stride = qs[0], os[0]
         p.qk_max, p.exp_sum, p.stats_mode = _ptr(qk_max), _ptr(exp_sum), stats_mode
+        return index
 
     def plan(self, query, out, key_cache, value_cache, key_scale, value_scale) -> None:
-        self._bind_fp8(query, out, key_cache, value_cache, key_scale, value_scale)
-        with _on(query.device):
-            rc = lib().pb_fp8_attn_plan(self._params_ref, self._cache_ref, _stream(query))
+        index = self._bind_fp8(query, out, key_cache, value_cache, key_scale, value_scale)
+        with _on(index):
+            rc = lib().pb_fp8_attn_plan(self._params_ref, self._cache_ref, torch._C._cuda_getCurrentRawStream(index))
         check(rc, "pb_fp8_attn_plan")
         self._planned = True
 
     def run(self, query, out, key_cache, value_cache, key_scale, value_scale, qk_max=None, exp_sum=None,
             stats_mode=_lib.PB_STATS_NONE):
         """One layer: attention of ``query`` over the cache into ``out``."""
-        self._bind_fp8(query, out, key_cache, value_cache, key_scale, value_scale, qk_max, exp_sum, stats_mode)
+        index = self._bind_fp8(query, out, key_cache, value_cache, key_scale, value_scale, qk_max, exp_sum, stats_mode)
         fn = lib().pb_fp8_attention_planned if self._planned else lib().pb_fp8_attention
-        with _on(query.device):
-            rc = fn(self._params_ref, self._cache_ref, _stream(query))
+        with _on(index):
+            rc = fn(self._params_ref, self._cache_ref, torch._C._cuda_getCurrentRawStream(index))
         if rc != _lib.PB_OK:
             check(rc, "pb_fp8_attention")
         return out

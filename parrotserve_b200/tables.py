@@ -11,8 +11,8 @@ from typing import NamedTuple, Optional
 import torch
 
 from ._lib import check, lib
-from .fp8 import _on
-from .ops import Workspace, _ptr, _require_cuda, _stream
+from .fp8 import _on, _one_device
+from .ops import Workspace, _ptr
 
 
 class BlockTables(NamedTuple):
@@ -45,36 +45,40 @@ def build_block_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, block
     ``kv_lens`` entry stays, ``num_failed`` counts it. Only ``block_tables`` is changed; the next iteration passes
     ``kv_lens`` and ``free_head`` of this one."""
     tensors = (context_lens, new_lens, block_tables, free_blocks, free_head) + (() if prefix_lens is None else (prefix_lens,))
-    _require_cuda(*tensors)
-    dev = context_lens.device
+    index = _one_device(*tensors)
     for t in tensors:
-        if t.dtype != torch.int32 or t.device != dev:
-            raise RuntimeError("lengths, tables and free blocks must be int32 tensors on one device")
-    if context_lens.dim() != 1 or new_lens.shape != context_lens.shape or (prefix_lens is not None and prefix_lens.shape != context_lens.shape):
+        if t.dtype != torch.int32:
+            raise RuntimeError("lengths, tables and free blocks must be int32 tensors")
+    shape, table_shape = context_lens.shape, block_tables.shape
+    if len(shape) != 1 or new_lens.shape != shape or (prefix_lens is not None and prefix_lens.shape != shape):
         raise RuntimeError("context_lens, new_lens and prefix_lens must be [num_requests]")
-    r = context_lens.shape[0]
-    if (block_tables.dim() != 2 or block_tables.shape[0] != r or (r and block_tables.shape[1] > 1 and block_tables.stride(1) != 1)
-            or free_blocks.dim() != 1 or free_head.numel() != 1):
-        raise RuntimeError("block_tables must be [num_requests, width] with dense rows, free_blocks [n], free_head one number")
+    r = shape[0]
+    if len(table_shape) != 2 or table_shape[0] != r or free_blocks.dim() != 1 or free_head.numel() != 1:
+        raise RuntimeError("block_tables must be [num_requests, width], free_blocks [n], free_head one number")
+    width, (table_stride, entry_stride) = table_shape[1], block_tables.stride()
+    if r and width > 1 and entry_stride != 1:
+        raise RuntimeError("the rows of block_tables must be dense")
     if not (context_lens.is_contiguous() and new_lens.is_contiguous() and free_blocks.is_contiguous()
             and (prefix_lens is None or prefix_lens.is_contiguous())):
         raise RuntimeError("lengths and free blocks must be contiguous")
     if not 0 <= num_prefills <= r or num_tokens < 0:
         raise RuntimeError("num_prefills must be at most the number of requests, num_tokens not negative")
-    width = block_tables.shape[1]
     # two allocations: the 64-bit and the 32-bit results
+    dev = context_lens.device
     longs = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
     sizes = (r + 1, r, 1, 1, num_tokens, num_tokens * width if with_suffix_tables else 0)
-    parts = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)
-    row_offsets, kv_lens, head_out, failed, suffix_lens, flat = parts
-    with _on(dev):
-        ws = Workspace.get(dev, lib().pb_block_tables_workspace_bytes(r))
+    ints = torch.empty(sum(sizes), dtype=torch.int32, device=dev)
+    row_offsets, kv_lens, head_out, failed, suffix_lens, flat = ints.split_with_sizes(sizes)
+    slot_mapping, positions = longs.unbind()
+    at64, at = longs.data_ptr(), ints.data_ptr()
+    with _on(index):
+        nbytes = lib().pb_block_tables_workspace_bytes(r)
+        ws = Workspace.get(dev, nbytes) if nbytes else None  # (up to some number of requests the call needs none)
         rc = lib().pb_build_block_tables(
-            context_lens.data_ptr(), new_lens.data_ptr(), r, block_tables.data_ptr(), width, block_tables.stride(0),
-            free_blocks.data_ptr(), free_blocks.shape[0], free_head.data_ptr(), _ptr(prefix_lens), block_size, num_prefills, num_tokens,
-            longs[0].data_ptr(), longs[1].data_ptr(), row_offsets.data_ptr(), kv_lens.data_ptr(), suffix_lens.data_ptr(),
-            flat.data_ptr() if with_suffix_tables else None, head_out.data_ptr(), failed.data_ptr(), ws.data_ptr(), ws.numel(),
-            _stream(context_lens))
+            context_lens.data_ptr(), new_lens.data_ptr(), r, block_tables.data_ptr(), width, table_stride, free_blocks.data_ptr(),
+            free_blocks.shape[0], free_head.data_ptr(), _ptr(prefix_lens), block_size, num_prefills, num_tokens, at64, at64 + 8 * num_tokens,
+            at, at + 4 * (r + 1), at + 4 * (2 * r + 3), at + 4 * (2 * r + 3 + num_tokens) if with_suffix_tables else None,
+            at + 4 * (2 * r + 1), at + 4 * (2 * r + 2), _ptr(ws), nbytes, torch._C._cuda_getCurrentRawStream(index))
     check(rc, "pb_build_block_tables")
-    return BlockTables(longs[0], longs[1], row_offsets, kv_lens, suffix_lens,
+    return BlockTables(slot_mapping, positions, row_offsets, kv_lens, suffix_lens,
                        flat.view(num_tokens, width) if with_suffix_tables else None, head_out, failed)

@@ -61,8 +61,10 @@ def test_fill_and_gather_refuse_bad_rows(args, code):
 
 def test_fill_needs_its_workspace():
     c = cache()
-    need = _lib.lib().pb_fp8_fill_workspace_bytes(3, 8, 16)
-    args = (FAKE, FAKE, FAKE, 1, 3, 512, 512, _lib.PB_F16)
+    assert _lib.lib().pb_fp8_fill_workspace_bytes(1024, 8, 16) == 0  # (the fill of few tokens reads the whole list)
+    need = _lib.lib().pb_fp8_fill_workspace_bytes(1025, 8, 16)
+    assert need > 0
+    args = (FAKE, FAKE, FAKE, 1, 1025, 512, 512, _lib.PB_F16)
     for ws, n in ((None, need), (FAKE, need - 1), (FAKE + 4, need)):
         assert _lib.lib().pb_fp8_reshape_and_cache(C.byref(c), *args, ws, n, None) == _lib.PB_ERR_WORKSPACE
     assert _lib.lib().pb_fp8_reshape_and_cache(C.byref(c), FAKE, FAKE, FAKE, 1, 0, 512, 512, _lib.PB_F16, None, 0, None) == _lib.PB_OK
@@ -118,8 +120,9 @@ GOOD_TABLES = dict(context_lens=FAKE, new_lens=FAKE, num_requests=3, block_table
     (dict(num_tokens=-1), _lib.PB_ERR_INVALID_ARG),
     (dict(block_size=0), _lib.PB_ERR_INVALID_ARG),
     (dict(table_stride=3), _lib.PB_ERR_INVALID_ARG),
-    (dict(workspace=None), _lib.PB_ERR_WORKSPACE),
-    (dict(workspace_bytes=8), _lib.PB_ERR_WORKSPACE),
+    (dict(num_requests=1025, workspace=None), _lib.PB_ERR_WORKSPACE),
+    (dict(num_requests=1025, workspace_bytes=8), _lib.PB_ERR_WORKSPACE),
+    (dict(num_requests=1025, workspace=FAKE + 4), _lib.PB_ERR_WORKSPACE),
 ])
 def test_block_table_refusals(over, code):
     a = {**GOOD_TABLES, **over}
