@@ -229,8 +229,116 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_rows_kernel(const Attn
   }
 }
 
+// Few (row, head) pairs that may have many partials, of a long context split over all SMs: a CTA per pair, its warps share the
+// partials. (One row of 100003 tokens x 64 heads in 98 chunks: 62 us of a pair's sixteen lanes, WIDE_US so.)
+constexpr int kWideWarps = 8, kWidePairs = 1024, kWideParts = 16;
+template <typename T, int D>
+__global__ void __launch_bounds__(kWideWarps * 32) merge_wide_kernel(const AttnDev d) {
+  constexpr int kThreads = kWideWarps * 32, kVecs = D / 4, kPer = (kVecs + 31) / 32;
+  __shared__ float weight[kThreads], red_m[kWideWarps], red_l[kWideWarps];
+  __shared__ float4 acc[kWideWarps][kVecs];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long long idx = blockIdx.x;
+  const int row = (int)(idx / d.num_heads), head = (int)(idx - (long long)row * d.num_heads);
+  const RowInfo info = d.row_info[row];
+  const PartCounts parts = count_parts(d, info, d.hdr[kHdrDnTiles], dense_ctas_of(d), head);
+  pdl_wait();  // as above
+  pdl_trigger();
+  if (idx == 0 && tid == 0) d.hdr[kHdrSqCounter] = 0;
+  const bool poison = call_failed(d);
+  if (parts.direct && !poison) return;
+  const int np = parts.prefix, nc = parts.segment, nsc = info.nsc, n = parts.direct ? 0 : np + nc + nsc + parts.outer;
+  auto slot_of = [&](int j) {
+    const int part = j < np ? j : j < np + nc ? d.pparts + (j - np) : j < np + nc + nsc ? d.pparts + d.cparts + (j - np - nc)
+                     : d.pparts + d.cparts + d.sparts + (j - np - nc - nsc);
+    return partial_slot(d, row, part, head);
+  };
+  float m_prev = -INFINITY, l_prev = 0.f;
+  if (d.stats_mode & PB_STATS_LOAD) {
+    m_prev = d.qk_max[idx];
+    l_prev = d.exp_sum[idx];
+    if (!(l_prev > 0.f)) { l_prev = 0.f; m_prev = -INFINITY; }
+  }
+  float M = m_prev;
+  for (int j = tid; j < n; j += kThreads) M = fmaxf(M, d.ml[slot_of(j)].x);
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if (lane == 0) red_m[warp] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWideWarps; ++w) M = fmaxf(M, red_m[w]);
+  const bool any = M > -INFINITY;
+  float4 o4[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) o4[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L = 0.f;
+  for (int jb = 0; any && jb < n; jb += kThreads) {
+    const int cnt = min(kThreads, n - jb);
+    if (jb > 0) __syncthreads();  // (the last round's weights have been read)
+    if (tid < cnt) {
+      const float2 ml = d.ml[slot_of(jb + tid)];
+      const float w = fast_exp2(ml.x - M);
+      weight[tid] = w;
+      L = fmaf(ml.y, w, L);
+    }
+    __syncthreads();
+    for (int j0 = warp; j0 < cnt; j0 += 4 * kWideWarps) {
+      float4 a[4][kPer];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u * kWideWarps;
+        const float4* ap = reinterpret_cast<const float4*>(d.acc + slot_of(jb + min(j, cnt - 1)) * D);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const int v = lane + 32 * k;
+          a[u][k] = (j < cnt && v < kVecs) ? __ldcs(ap + v) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u * kWideWarps;
+        const float w = j < cnt ? weight[j] : 0.f;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          o4[k].x = fmaf(a[u][k].x, w, o4[k].x); o4[k].y = fmaf(a[u][k].y, w, o4[k].y);
+          o4[k].z = fmaf(a[u][k].z, w, o4[k].z); o4[k].w = fmaf(a[u][k].w, w, o4[k].w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  if (lane == 0) red_l[warp] = L;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k)
+    if (lane + 32 * k < kVecs) acc[warp][lane + 32 * k] = o4[k];
+  __syncthreads();
+  L = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWideWarps; ++w) L += red_l[w];
+  const float w_prev = l_prev > 0.f ? fast_exp2(m_prev - M) * l_prev : 0.f;
+  L += w_prev;
+  const float inv = poison ? __int_as_float(0x7fc00000) : (L > 0.f) ? 1.f / L : 0.f;
+  T* op = reinterpret_cast<T*>(d.out) + (size_t)row * d.out_stride + (size_t)head * D;
+  for (int i = tid; i < D; i += kThreads) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWideWarps; ++w) v += reinterpret_cast<const float*>(acc[w])[i];
+    if (l_prev > 0.f) v = fmaf(to_float<T>(op[i]), w_prev, v);
+    op[i] = from_float<T>(v * inv);
+  }
+  if ((d.stats_mode & PB_STATS_SAVE) && tid == 0) {
+    d.qk_max[idx] = M;
+    d.exp_sum[idx] = L;
+  }
+}
+
 template <typename T, int D>
 cudaError_t launch_merge_d(const AttnDev& d, cudaStream_t s) {
+  // (of the 8-bit cache's calls: with the 16-bit one a sum keeps its order)
+  const long long pairs = (long long)d.num_rows * d.num_heads;
+  if (d.key_scale && pairs <= kWidePairs && d.pparts + d.cparts + d.sparts >= kWideParts)
+    return launch_kernel(merge_wide_kernel<T, D>, (unsigned)pairs, kWideWarps * 32, 0, s, true, d);
   if (d.seg_rows_max >= kManyRows) {  // (only prefill rows are ever finished before; decode rows do not count)
     const int hpc = d.num_heads < kMaxHeadsPerCta ? d.num_heads : kMaxHeadsPerCta;
     const unsigned grid = (unsigned)((long long)d.num_rows * ((d.num_heads + hpc - 1) / hpc));
