@@ -66,8 +66,8 @@ struct DecCtl {
   DecDesc desc[kDescSlots];
   DecItem item[kItemSlots];
   float mul[2][8];               // per query operand slot and head: scale * log2(e) / (power of two of the row)
-  float xmax[2][4][8];           // exchange between the softmax warps
-  float xsum[2][4][8];
+  float4 xmax[2][8];             // exchange between the softmax warps: per head, the warps' numbers
+  float4 xsum[2][8];
   uint64_t full[8], empty[8];    // stages
   uint64_t desc_full[kDescSlots], desc_empty[kDescSlots], item_full[kItemSlots], item_empty[kItemSlots];
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], pv_done[2], exchange;
@@ -111,6 +111,33 @@ __device__ __forceinline__ void parts_of(float x, uint32_t (&p)[kParts]) {
     p[i] = fp8::pack2(x, 0.f);
     if (i < kParts - 1) x = (x - fp8::to_float2(p[i]).x) * 16.f;
   }
+}
+// The same of two numbers (low and second bytes). What two parts leave, 2^-8 of x, needs no more than fp16.
+__device__ __forceinline__ void parts_of_two(float x, float y, uint32_t (&p)[kParts]) {
+  p[0] = fp8::pack2(x, y);
+  float2 a = fp8::to_float2(p[0]);
+  x = (x - a.x) * 16.f; y = (y - a.y) * 16.f;
+  p[1] = fp8::pack2(x, y);
+  a = fp8::to_float2(p[1]);
+  __half2 r = __floats2half2_rn((x - a.x) * 16.f, (y - a.y) * 16.f);
+  p[2] = fp8::pack2(r);
+  const uint32_t b = fp8::to_half2(p[2]);
+  r = __hmul2(__hsub2(r, *reinterpret_cast<const __half2*>(&b)), __float2half2_rn(16.f));
+  p[3] = fp8::pack2(r);
+}
+// Maximum over a warp (NaN counts as nothing, like fmaxf).
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+__device__ __forceinline__ float max4(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+// Lane h < N leaves v[h] (the same in all lanes) as warp w's number of head h.
+template <int N> __device__ __forceinline__ void leave(float4* to, const float (&v)[N], int w, int lane) {
+  float mine = v[0];
+#pragma unroll
+  for (int h = 1; h < N; ++h) mine = lane == h ? v[h] : mine;
+  if (lane < N) reinterpret_cast<float*>(to + lane)[w] = mine;
 }
 // The sum of the parts' columns of head h.
 template <int HMAX> __device__ __forceinline__ float join_parts(const uint32_t* c, int h) {
@@ -508,14 +535,10 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
         top[h] = seen ? lg[h] + fmaxf(lv, kMinLv) : -INFINITY;  // (a block without a scale: no weight, but a reference)
       }
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1)
-#pragma unroll
-        for (int h = 0; h < HMAX; ++h) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+      for (int h = 0; h < HMAX; ++h) top[h] = warp_max(top[h]);
       // the tile's maximum, from the four warps
       const int xb = x_use & 1;
-#pragma unroll
-      for (int h = 0; h < HMAX; ++h)
-        if (lane == h) ctl.xmax[xb][warp][h] = top[h];
+      leave(ctl.xmax[xb], top, warp, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(ctl.exchange));
       if (!wait_or_abort(bar(ctl.exchange), x_use & 1, abort_flag, status)) break;
@@ -524,7 +547,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
       float alpha[HMAX];
 #pragma unroll
       for (int h = 0; h < HMAX; ++h) {
-        const float m = fmaxf(fmaxf(ctl.xmax[xb][0][h], ctl.xmax[xb][1][h]), fmaxf(ctl.xmax[xb][2][h], ctl.xmax[xb][3][h]));
+        const float m = max4(ctl.xmax[xb][h]);
         alpha[h] = 1.f;
         if (m > ref[h] + kLag) {
           alpha[h] = fast_exp2(ref[h] - m);
@@ -548,16 +571,28 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
         tmem_wait_st();
       }
       uint8_t* wop = smem + C::kOffW + buf * C::kW + blk_of * (C::kN * 16) + (r & 15);
+      float w[HMAX];
 #pragma unroll
       for (int h = 0; h < HMAX; ++h) {
         const float base = ref[h] == -INFINITY ? 0.f : ref[h];  // (nothing but logits of -inf so far)
         l[h] += fast_exp2(lg[h] - base);
-        uint32_t p[kParts];
-        parts_of(fast_exp2(lg[h] + (lv - base + kTop)), p);
+        w[h] = fast_exp2(lg[h] + (lv - base + kTop));
+      }
+      auto put = [&](int n, uint32_t code) { wop[(n >> 3) * 128 + (n & 7) * 16] = (uint8_t)code; };
+      uint32_t p[kParts];
+      if constexpr (HMAX == 1) {
+        parts_of(w[0], p);
 #pragma unroll
-        for (int i = 0; i < kParts; ++i) {
-          const int n = i * HMAX + h;
-          wop[(n >> 3) * 128 + (n & 7) * 16] = (uint8_t)p[i];
+        for (int i = 0; i < kParts; ++i) put(i, p[i]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < HMAX; h += 2) {
+          parts_of_two(w[h], w[h + 1], p);
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) {
+            put(i * HMAX + h, p[i]);
+            put(i * HMAX + h + 1, p[i] >> 8);
+          }
         }
       }
       if ((ntok & 31) && r < D) {
@@ -584,17 +619,12 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
       // ---- the item's partial: sums and exact maxima from the four warps, O from tensor memory ----
 #pragma unroll
       for (int h = 0; h < HMAX; ++h) {
-        float sum = l[h], m = mx[h];
+        mx[h] = warp_max(mx[h]);
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        }
-        if (lane == h) {
-          ctl.xsum[x_use & 1][warp][h] = sum;
-          ctl.xmax[x_use & 1][warp][h] = m;
-        }
+        for (int o = 16; o >= 1; o >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
       }
+      leave(ctl.xmax[x_use & 1], mx, warp, lane);
+      leave(ctl.xsum[x_use & 1], l, warp, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(ctl.exchange));
       if (!wait_or_abort(bar(ctl.exchange), x_use & 1, abort_flag, status)) break;
@@ -609,8 +639,9 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
 #pragma unroll
       for (int h = 0; h < HMAX; ++h) {
         if (h < hpi) {
-          const float m = fmaxf(fmaxf(ctl.xmax[eb][0][h], ctl.xmax[eb][1][h]), fmaxf(ctl.xmax[eb][2][h], ctl.xmax[eb][3][h]));
-          const float sum = (ctl.xsum[eb][0][h] + ctl.xsum[eb][1][h]) + (ctl.xsum[eb][2][h] + ctl.xsum[eb][3][h]);
+          const float m = max4(ctl.xmax[eb][h]);
+          const float4 sums = ctl.xsum[eb][h];
+          const float sum = (sums.x + sums.y) + (sums.z + sums.w);
           const float fix = ref[h] == -INFINITY ? 0.f : fast_exp2(ref[h] - m);
           const float v = join_parts<HMAX>(o, h);
           const size_t slot = partial_slot(d, row, part, head + h);

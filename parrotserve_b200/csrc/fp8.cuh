@@ -26,6 +26,9 @@ __device__ __forceinline__ float scaled(float x, float inv) { return fabsf(x) <=
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ uint32_t pack2(__half2 v) {
+  return (uint32_t)__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(v), __NV_SATFINITE, __NV_E4M3);
+}
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return pack2(a, b) | (pack2(c, d) << 16); }
 
 // The smallest power of two s with top <= 448 * s (448 = 1.75 * 2^8), from 2^-126 on; 0 for 0. top is finite, >= 0.
