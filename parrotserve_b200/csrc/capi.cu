@@ -317,7 +317,7 @@ pb_attn_params with_fp8_chunks(const pb_attn_params* p) {
   pb_attn_params q = *p;
   if (q.suffix_chunk_blocks <= 0 && decode_fp8_supported(q.dtype, q.head_size, q.block_size) && q.num_heads > 0 && q.num_rows > 0) {
     const int share = heads_per_item(&q);
-    const long long ctas = (long long)sm_count() * (share > 4 ? 2 : 3);
+    const long long ctas = (long long)sm_count() * (share > 1 ? 2 : 3);
     const long long blocks = (long long)q.num_rows * (q.num_heads / share) * q.suffix_table_stride / 2;
     const int cs = pow2_floor(blocks / (2 * ctas) > 0 ? blocks / (2 * ctas) : 1);
     q.suffix_chunk_blocks = cs < 8 ? 8 : cs > 128 ? 128 : cs;

@@ -9,7 +9,7 @@
 // writes the weight's parts back. A part is an e4m3 value, the rounded remainder of those before it, times 16 more each:
 //     x = x0 + x1 / 16 + x2 / 256 + x3 / 4096: off by 2^-16 of itself or by half a step of x3, 2^-22 (q is scaled by a
 //     power of two to a largest element in [2^7, 2^8), the largest weight of a row lies in [2^8, 2^8.75))
-// Column p * HMAX + h holds part p of query head h of the item (up to HMAX heads of one kv head).
+// With up to HMAX heads of one kv head in an item, column (g * kParts + p) * kHeads + h holds part p of head h of the g-th kHeads.
 // Operand layouts (no swizzle, K-major, 8 x 16-byte core matrices): V tiles are made of them as they lie in the cache, [d][16 tok];
 // the 256-byte chunk rows of the K tiles are put side by side, [d chunk][block][16 tok], by per-thread 16-byte async copies.
 //
@@ -32,7 +32,6 @@ namespace {
 using namespace dense;
 using fp8::kMinLv;
 
-constexpr int kDecThreads = 288;
 constexpr int kDescSlots = 4, kItemSlots = 4;
 constexpr int kParts = 4;                  // the MMA takes sixteen columns or none: four parts cost what three do
 constexpr float kTop = 8.f, kLag = 0.75f;  // the largest weight of a row lies in [2^kTop, 2^(kTop + kLag)) < 448
@@ -53,8 +52,12 @@ struct DecCfg {
   static constexpr int kN = HMAX > 4 ? 32 : 16;       // columns: kParts * HMAX, in sixteens
   static constexpr int kTile = D * 16;                // one K or V tile of a (block, head)
   static constexpr int kStage = 2 * 8 * kTile;        // K, then V
-  static constexpr int kCtas = HMAX > 4 ? 2 : 3;      // per SM
-  static constexpr int kStages = HMAX > 4 ? (D == 128 ? 2 : D == 96 ? 3 : 5) : 2 * 128 / D;
+  static constexpr int kGroups = HMAX > 1 ? 2 : 1;    // softmax groups of four warps; each has all tokens and
+  static constexpr int kHeads = HMAX / kGroups;       // so many of the heads
+  static constexpr int kW0 = 4 * kGroups;             // the first warp behind them
+  static constexpr int kThreads = 32 * (kW0 + 5);
+  static constexpr int kCtas = HMAX > 1 ? 2 : 3;      // per SM
+  static constexpr int kStages = HMAX == 1 ? 2 * 128 / D : HMAX == 4 ? 3 * 128 / D : D == 128 ? 2 : D == 96 ? 3 : 5;
   static constexpr int kQ = kN * D, kW = kN * 128;    // operands of one item / one tile
   // rows of V beyond D (the MMA always has 128) are read from what lies behind the tile: kPad bytes behind the last stage
   static constexpr int kPad = (128 - D) * 16;
@@ -66,11 +69,11 @@ struct DecCtl {
   DecDesc desc[kDescSlots];
   DecItem item[kItemSlots];
   float mul[2][8];               // per query operand slot and head: scale * log2(e) / (power of two of the row)
-  float4 xmax[2][8];             // exchange between the softmax warps: per head, the warps' numbers
-  float4 xsum[2][8];
+  float4 xmax[2][2][4];          // exchange between the softmax warps of a group: per head, the warps' numbers
+  float4 xsum[2][2][4];
   uint64_t full[8], empty[8];    // stages
   uint64_t desc_full[kDescSlots], desc_empty[kDescSlots], item_full[kItemSlots], item_empty[kItemSlots];
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], pv_done[2], exchange;
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], pv_done[2], exchange[2];
   uint32_t tmem;
   int abort_flag;
 };
@@ -87,21 +90,28 @@ __device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t* v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
                ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
-// The kParts * HMAX columns of parts, in registers.
-template <int HMAX> struct Cols { static constexpr int kRegs = HMAX == 1 ? 4 : HMAX == 4 ? 16 : 32; };
-template <int HMAX> __device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t* v) {
-  if constexpr (HMAX == 1) tmem_ld4(taddr, v);
-  else if constexpr (HMAX == 4) tmem_ld16(taddr, v);
-  else tmem_ld32(taddr, v);
+// The kParts * N columns of parts of a group's N heads, in registers.
+template <int N> __device__ __forceinline__ void ld_cols(uint32_t taddr, uint32_t* v) {
+  if constexpr (N == 1) tmem_ld4(taddr, v);
+  else if constexpr (N == 2) tmem_ld8(taddr, v);
+  else tmem_ld16(taddr, v);
 }
-template <int HMAX> __device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t* v) {
-  if constexpr (HMAX == 1) tmem_st4(taddr, v);
-  else if constexpr (HMAX == 4) tmem_st16(taddr, v);
-  else tmem_st32(taddr, v);
+template <int N> __device__ __forceinline__ void st_cols(uint32_t taddr, const uint32_t* v) {
+  if constexpr (N == 1) tmem_st4(taddr, v);
+  else if constexpr (N == 2) tmem_st8(taddr, v);
+  else tmem_st16(taddr, v);
 }
 
 // x -> its parts as codes (low bytes).
@@ -139,11 +149,11 @@ template <int N> __device__ __forceinline__ void leave(float4* to, const float (
   for (int h = 1; h < N; ++h) mine = lane == h ? v[h] : mine;
   if (lane < N) reinterpret_cast<float*>(to + lane)[w] = mine;
 }
-// The sum of the parts' columns of head h.
-template <int HMAX> __device__ __forceinline__ float join_parts(const uint32_t* c, int h) {
-  float sum = __uint_as_float(c[(kParts - 1) * HMAX + h]);
+// The sum of the parts' columns of a group's head h.
+template <int N> __device__ __forceinline__ float join_parts(const uint32_t* c, int h) {
+  float sum = __uint_as_float(c[(kParts - 1) * N + h]);
 #pragma unroll
-  for (int i = kParts - 2; i >= 0; --i) sum = fmaf(sum, 1.f / 16, __uint_as_float(c[i * HMAX + h]));
+  for (int i = kParts - 2; i >= 0; --i) sum = fmaf(sum, 1.f / 16, __uint_as_float(c[i * N + h]));
   return sum;
 }
 
@@ -155,7 +165,7 @@ struct DecClaim {
 };
 
 template <typename T, int D, int HMAX>
-__global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_fp8_kernel(const AttnDev d) {
+__global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>::kCtas)) decode_fp8_kernel(const AttnDev d) {
   using C = DecCfg<D, HMAX>;
   extern __shared__ __align__(1024) uint8_t smem[];
   DecCtl& ctl = *reinterpret_cast<DecCtl*>(smem + C::kOffCtl);
@@ -179,17 +189,17 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(ctl.q_full[i]), 32);
-      mbar_init(bar(ctl.q_empty[i]), 1 + 4);  // the MMAs that read it, the softmax warps (its factors)
+      mbar_init(bar(ctl.q_empty[i]), 1 + C::kW0);  // the MMAs that read it, the softmax warps (its factors)
       mbar_init(bar(ctl.s_full[i]), 1);
-      mbar_init(bar(ctl.p_full[i]), 128);
+      mbar_init(bar(ctl.p_full[i]), 32 * C::kW0);
       mbar_init(bar(ctl.pv_done[i]), 1);
+      mbar_init(bar(ctl.exchange[i]), 4);
     }
-    mbar_init(bar(ctl.exchange), 4);
     ctl.abort_flag = 0;
     mbar_fence_init();
     fence_proxy_async_smem();
   }
-  if (warp == 7) tmem_alloc(smem_u32(&ctl.tmem), C::kTmem);
+  if (warp == C::kW0 + 3) tmem_alloc(smem_u32(&ctl.tmem), C::kTmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -200,14 +210,14 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
   if constexpr (HMAX > 1) {
     const int share = d.num_heads / d.num_kv_heads;
     bool usual = true;
-    for (int h = threadIdx.x; h < d.num_heads; h += kDecThreads) usual = usual && d.head_mapping[h] == h / share;
+    for (int h = threadIdx.x; h < d.num_heads; h += C::kThreads) usual = usual && d.head_mapping[h] == h / share;
     if (__syncthreads_and(usual)) hpi = d.gqa_heads;
   }
   const uint32_t tmem = ctl.tmem;
   const uint32_t tmem_s = tmem, tmem_o = tmem + 2 * C::kN;
   const uint32_t stage0 = smem_u32(smem);
 
-  if (warp == 4) {
+  if (warp == C::kW0) {
     // ================= lister: items, tiles, V =================
     const int H = d.num_heads / hpi;
     const long long n_items = (long long)d.hdr[kHdrNumSq] * H;
@@ -337,7 +347,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
       for (uint32_t c = tc > C::kStages ? tc - C::kStages : 0; c < tc; ++c)
         (void)mbar_wait_bounded(bar(ctl.full[c % C::kStages]), (c / C::kStages) & 1);
     }
-  } else if (warp == 5 || warp == 6) {
+  } else if (warp == C::kW0 + 1 || warp == C::kW0 + 2) {
     // ================= K: 16-byte async copies, the chunk rows of the tile's blocks side by side =================
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(d.key_cache);
     for (uint32_t tc = 0;; ++tc) {
@@ -347,7 +357,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
       const int nb = e.nb;
       if (nb == 0) break;
       if (tc >= C::kStages && !wait_or_abort(bar(ctl.empty[s]), ((tc / C::kStages) & 1) ^ 1, abort_flag, status)) break;
-      for (int j = warp - 5; j < nb; j += 2) {
+      for (int j = warp - C::kW0 - 1; j < nb; j += 2) {
         const uint8_t* src = kc + (size_t)e.blk[j] * d.kv_block_stride + (size_t)e.kvh * d.kv_head_stride + lane * 16;
         const uint32_t dst = stage0 + s * C::kStage + (lane >> 4) * 2048 + j * 256 + (lane & 15) * 16;
 #pragma unroll
@@ -356,7 +366,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
       cp_async_arrive_noinc(bar(ctl.full[s]));
     }
     cp_async_wait_all();
-  } else if (warp == 8) {
+  } else if (warp == C::kW0 + 4) {
     // ================= query operands =================
     const uint8_t* qg = reinterpret_cast<const uint8_t*>(d.query);
     for (uint32_t ic = 0;; ++ic) {
@@ -402,7 +412,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
           const uint32_t lo = fp8::pack2(f[0], f[1]), hi = fp8::pack2(f[2], f[3]);
           const float2 a = fp8::to_float2(lo), b = fp8::to_float2(hi);
           f[0] = (f[0] - a.x) * 16.f; f[1] = (f[1] - a.y) * 16.f; f[2] = (f[2] - b.x) * 16.f; f[3] = (f[3] - b.y) * 16.f;
-          const int n = p * HMAX + h;
+          const int n = (h / C::kHeads * kParts + p) * C::kHeads + h % C::kHeads;
           if (lane < D / 4)
             *reinterpret_cast<uint32_t*>(qop + (lane >> 2) * (C::kN * 16) + (n >> 3) * 128 + (n & 7) * 16 + (lane & 3) * 4) = lo | (hi << 16);
         }
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
       fence_proxy_async_smem();
       mbar_arrive(bar(ctl.q_full[slot]));
     }
-  } else if (warp == 7) {
+  } else if (warp == C::kW0 + 3) {
     // ================= MMA issuer =================
     // S(t + 1) as soon as its tile is there, O(t) as soon as its weights are: whichever comes first.
     constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(C::kN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);  // fp32 += e4m3 . e4m3
@@ -497,13 +507,15 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
     }
   } else {
     // ================= softmax (a token per thread) and epilogue (an element d per thread) =================
-    const int r = warp * 32 + lane;
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    constexpr int N = C::kHeads;
+    const int g = warp >> 2, quarter = warp & 3, h0 = g * N;  // the group's first head
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_base = ((uint32_t)(quarter * 32) << 16) + g * kParts * N;  // (and its columns)
     const int blk_of = r >> 4;
-    float mul[HMAX], ref[HMAX], l[HMAX], mx[HMAX];
+    float mul[N], ref[N], l[N], mx[N];
     uint32_t items = 0, x_use = 0;
 #pragma unroll
-    for (int h = 0; h < HMAX; ++h) { mul[h] = 0.f; ref[h] = -INFINITY; l[h] = 0.f; mx[h] = -INFINITY; }
+    for (int h = 0; h < N; ++h) { mul[h] = 0.f; ref[h] = -INFINITY; l[h] = 0.f; mx[h] = -INFINITY; }
     for (uint32_t tc = 0;; ++tc) {
       const int rr = tc % kDescSlots, s = tc % C::kStages, buf = tc & 1;
       if (!wait_or_abort(bar(ctl.desc_full[rr]), (tc / kDescSlots) & 1, abort_flag, status)) break;
@@ -516,38 +528,38 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
         const int slot = items & 1;
         if (!wait_or_abort(bar(ctl.q_full[slot]), (items >> 1) & 1, abort_flag, status)) break;
 #pragma unroll
-        for (int h = 0; h < HMAX; ++h) { mul[h] = ctl.mul[slot][h]; ref[h] = -INFINITY; l[h] = 0.f; mx[h] = -INFINITY; }
+        for (int h = 0; h < N; ++h) { mul[h] = ctl.mul[slot][h0 + h]; ref[h] = -INFINITY; l[h] = 0.f; mx[h] = -INFINITY; }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(ctl.q_empty[slot]));
         ++items;
       }
       if (!wait_or_abort(bar(ctl.s_full[buf]), (tc >> 1) & 1, abort_flag, status)) break;
       tc_fence_after();
-      uint32_t c[Cols<HMAX>::kRegs];
-      ld_cols<HMAX>(tmem_s + buf * C::kN + lane_base, c);
+      uint32_t c[kParts * N];
+      ld_cols<N>(tmem_s + buf * C::kN + lane_base, c);
       tmem_wait_ld();
       const bool seen = r < ntok;
-      float lg[HMAX], top[HMAX];
+      float lg[N], top[N];
 #pragma unroll
-      for (int h = 0; h < HMAX; ++h) {
-        lg[h] = seen ? join_parts<HMAX>(c, h) * (ks * mul[h]) : -INFINITY;
+      for (int h = 0; h < N; ++h) {
+        lg[h] = seen ? join_parts<N>(c, h) * (ks * mul[h]) : -INFINITY;
         mx[h] = fmaxf(mx[h], lg[h]);
         top[h] = seen ? lg[h] + fmaxf(lv, kMinLv) : -INFINITY;  // (a block without a scale: no weight, but a reference)
       }
 #pragma unroll
-      for (int h = 0; h < HMAX; ++h) top[h] = warp_max(top[h]);
+      for (int h = 0; h < N; ++h) top[h] = warp_max(top[h]);
       // the tile's maximum, from the four warps
       const int xb = x_use & 1;
-      leave(ctl.xmax[xb], top, warp, lane);
+      leave(ctl.xmax[g][xb], top, quarter, lane);
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(ctl.exchange));
-      if (!wait_or_abort(bar(ctl.exchange), x_use & 1, abort_flag, status)) break;
+      if (lane == 0) mbar_arrive(bar(ctl.exchange[g]));
+      if (!wait_or_abort(bar(ctl.exchange[g]), x_use & 1, abort_flag, status)) break;
       ++x_use;
       bool grow = false;
-      float alpha[HMAX];
+      float alpha[N];
 #pragma unroll
-      for (int h = 0; h < HMAX; ++h) {
-        const float m = max4(ctl.xmax[xb][h]);
+      for (int h = 0; h < N; ++h) {
+        const float m = max4(ctl.xmax[g][xb][h]);
         alpha[h] = 1.f;
         if (m > ref[h] + kLag) {
           alpha[h] = fast_exp2(ref[h] - m);
@@ -556,46 +568,50 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
         }
         l[h] *= alpha[h];
       }
-      if (grow && !first) {  // (the same for all four warps) the accumulator follows, once the previous tile is in it
+      if (grow && !first) {  // (the same for all warps of the group) the accumulator follows, once the previous tile is in it
         if (!wait_or_abort(bar(ctl.pv_done[buf ^ 1]), ((tc - 1) >> 1) & 1, abort_flag, status)) break;
         tc_fence_after();
-        uint32_t o[Cols<HMAX>::kRegs];
+        uint32_t o[kParts * N];
         const uint32_t at = tmem_o + ((items - 1) & 1) * C::kN + lane_base;
-        ld_cols<HMAX>(at, o);
+        ld_cols<N>(at, o);
         tmem_wait_ld();
 #pragma unroll
-        for (int h = 0; h < HMAX; ++h)
+        for (int h = 0; h < N; ++h)
 #pragma unroll
-          for (int p = 0; p < kParts; ++p) o[p * HMAX + h] = __float_as_uint(__uint_as_float(o[p * HMAX + h]) * alpha[h]);
-        st_cols<HMAX>(at, o);
+          for (int p = 0; p < kParts; ++p) o[p * N + h] = __float_as_uint(__uint_as_float(o[p * N + h]) * alpha[h]);
+        st_cols<N>(at, o);
         tmem_wait_st();
       }
       uint8_t* wop = smem + C::kOffW + buf * C::kW + blk_of * (C::kN * 16) + (r & 15);
-      float w[HMAX];
+      const int n0 = g * kParts * N;  // the group's first column
+      float w[N];
 #pragma unroll
-      for (int h = 0; h < HMAX; ++h) {
+      for (int h = 0; h < N; ++h) {
         const float base = ref[h] == -INFINITY ? 0.f : ref[h];  // (nothing but logits of -inf so far)
         l[h] += fast_exp2(lg[h] - base);
         w[h] = fast_exp2(lg[h] + (lv - base + kTop));
       }
-      auto put = [&](int n, uint32_t code) { wop[(n >> 3) * 128 + (n & 7) * 16] = (uint8_t)code; };
+      auto put = [&](int i, uint32_t code) {
+        const int n = n0 + i;
+        wop[(n >> 3) * 128 + (n & 7) * 16] = (uint8_t)code;
+      };
       uint32_t p[kParts];
-      if constexpr (HMAX == 1) {
+      if constexpr (N == 1) {
         parts_of(w[0], p);
 #pragma unroll
         for (int i = 0; i < kParts; ++i) put(i, p[i]);
       } else {
 #pragma unroll
-        for (int h = 0; h < HMAX; h += 2) {
+        for (int h = 0; h < N; h += 2) {
           parts_of_two(w[h], w[h + 1], p);
 #pragma unroll
           for (int i = 0; i < kParts; ++i) {
-            put(i * HMAX + h, p[i]);
-            put(i * HMAX + h + 1, p[i] >> 8);
+            put(i * N + h, p[i]);
+            put(i * N + h + 1, p[i] >> 8);
           }
         }
       }
-      if ((ntok & 31) && r < D) {
+      if ((ntok & 31) && r < D && g == 0) {
         // the last 32 tokens are not all there: clear the codes behind the context (0 * NaN would not be 0)
         if (!wait_or_abort(bar(ctl.full[s]), (tc / C::kStages) & 1, abort_flag, status)) break;
         uint8_t* v = smem + s * C::kStage + 8 * C::kTile + r * 16;
@@ -618,33 +634,33 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
 
       // ---- the item's partial: sums and exact maxima from the four warps, O from tensor memory ----
 #pragma unroll
-      for (int h = 0; h < HMAX; ++h) {
+      for (int h = 0; h < N; ++h) {
         mx[h] = warp_max(mx[h]);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
       }
-      leave(ctl.xmax[x_use & 1], mx, warp, lane);
-      leave(ctl.xsum[x_use & 1], l, warp, lane);
+      leave(ctl.xmax[g][x_use & 1], mx, quarter, lane);
+      leave(ctl.xsum[g][x_use & 1], l, quarter, lane);
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(ctl.exchange));
-      if (!wait_or_abort(bar(ctl.exchange), x_use & 1, abort_flag, status)) break;
+      if (lane == 0) mbar_arrive(bar(ctl.exchange[g]));
+      if (!wait_or_abort(bar(ctl.exchange[g]), x_use & 1, abort_flag, status)) break;
       const int eb = x_use & 1;
       ++x_use;
       if (!wait_or_abort(bar(ctl.pv_done[buf]), (tc >> 1) & 1, abort_flag, status)) break;
       tc_fence_after();
-      uint32_t o[Cols<HMAX>::kRegs];
-      ld_cols<HMAX>(tmem_o + ((items - 1) & 1) * C::kN + lane_base, o);
+      uint32_t o[kParts * N];
+      ld_cols<N>(tmem_o + ((items - 1) & 1) * C::kN + lane_base, o);
       tmem_wait_ld();
       tc_fence_before();
 #pragma unroll
-      for (int h = 0; h < HMAX; ++h) {
-        if (h < hpi) {
-          const float m = max4(ctl.xmax[eb][h]);
-          const float4 sums = ctl.xsum[eb][h];
+      for (int h = 0; h < N; ++h) {
+        if (h0 + h < hpi) {
+          const float m = max4(ctl.xmax[g][eb][h]);
+          const float4 sums = ctl.xsum[g][eb][h];
           const float sum = (sums.x + sums.y) + (sums.z + sums.w);
           const float fix = ref[h] == -INFINITY ? 0.f : fast_exp2(ref[h] - m);
-          const float v = join_parts<HMAX>(o, h);
-          const size_t slot = partial_slot(d, row, part, head + h);
+          const float v = join_parts<N>(o, h);
+          const size_t slot = partial_slot(d, row, part, head + h0 + h);
           if (r < D) d.acc[slot * D + r] = v * (fix * (1.f / 256));  // (2^-kTop)
           if (r == 0) d.ml[slot] = make_float2(m, sum * fix);
         }
@@ -654,7 +670,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecCfg<D, HMAX>::kCtas)) decode_
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 7) {
+  if (warp == C::kW0 + 3) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kTmem);
   }
@@ -670,7 +686,7 @@ cudaError_t launch_dec(const AttnDev& d, cudaStream_t s) {
   auto kfn = decode_fp8_kernel<T, D, HMAX>;
   cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kfn, d.num_sms * C::kCtas, kDecThreads, smem, s, true, d);
+  return launch_kernel(kfn, d.num_sms * C::kCtas, C::kThreads, smem, s, true, d);
 }
 
 template <typename T>
