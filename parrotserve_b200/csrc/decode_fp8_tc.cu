@@ -18,8 +18,8 @@
 // spend about 100 instructions each on eight of them. What bounds it now is memory.
 //
 // Three CTAs an SM (two with more than four heads per item), so that the copies of one run under the chain of another.
-// Warps 0-3 softmax and epilogue, warp 4 claims items, lists their tiles and copies V, warps 5, 6 copy K, warp 7 issues the
-// MMAs, warp 8 makes the query operands. Every mbarrier wait is bounded; on expiry the CTA records a status, drains and returns.
+// Warps 0-3 softmax and epilogue, behind them one warp claims items and lists their tiles, two copy K
+// (one of them V too), one issues the MMAs and one makes the query operands. Every mbarrier wait is bounded; on expiry the CTA records a status, drains and returns.
 #include <type_traits>
 
 #include "common.cuh"
@@ -32,7 +32,7 @@ namespace {
 using namespace dense;
 using fp8::kMinLv;
 
-constexpr int kDescSlots = 4, kItemSlots = 4;
+constexpr int kDescSlots = 8, kItemSlots = 4;  // (how far the lister runs ahead: it waits for three loads in a row per item)
 constexpr int kParts = 4;                  // the MMA takes sixteen columns or none: four parts cost what three do
 constexpr float kTop = 8.f, kLag = 0.75f;  // the largest weight of a row lies in [2^kTop, 2^(kTop + kLag)) < 448
 
@@ -70,7 +70,9 @@ struct DecCtl {
   DecItem item[kItemSlots];
   float mul[2][8];               // per query operand slot and head: scale * log2(e) / (power of two of the row)
   float4 xmax[2][2][4];          // exchange between the softmax warps of a group: per head, the warps' numbers
-  float4 xsum[2][2][4];
+  float4 left_max[2][2][4], left_sum[2][2][4];  // per group and item: what the warps leave for its epilogue
+  float left_ref[2][2][4];
+  int left_row[2][2], left_head[2][2], left_part[2][2];
   uint64_t full[8], empty[8];    // stages
   uint64_t desc_full[kDescSlots], desc_empty[kDescSlots], item_full[kItemSlots], item_empty[kItemSlots];
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], pv_done[2], exchange[2];
@@ -265,8 +267,6 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
       vs = d.value_scale[o];
     };
     auto claim = [&]() { return lane == 0 ? atomicAdd(&d.hdr[kHdrSqCounter], 1) : 0; };
-    const uint64_t policy = l2_policy_evict_first();
-    const uint8_t* vc = reinterpret_cast<const uint8_t*>(d.value_cache);
     uint32_t tc = 0, ic = 0;
     bool ok = true;
     DecClaim cur = describe(__shfl_sync(0xffffffffu, claim(), 0));
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
           scales_of(cur, b0, ids, ks, vs);
         }
         const int nb = min(8, cur.nblk - b0);
-        const int s = tc % C::kStages, r = tc % kDescSlots;
+        const int r = tc % kDescSlots;
         if (tc >= kDescSlots && !wait_or_abort(bar(ctl.desc_empty[r]), ((tc / kDescSlots) & 1) ^ 1, abort_flag, status)) { ok = false; break; }
         const int src = (b0 & 31) + (lane & 7);
         const int blk = __shfl_sync(0xffffffffu, ids, src);
@@ -313,12 +313,6 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
           e.last = b0 + 8 >= cur.nblk;
         }
         mbar_arrive(bar(ctl.desc_full[r]));
-        if (tc >= C::kStages && !wait_or_abort(bar(ctl.empty[s]), ((tc / C::kStages) & 1) ^ 1, abort_flag, status)) { ok = false; break; }
-        if (lane == 0) mbar_arrive_expect_tx(bar(ctl.full[s]), nb * C::kTile);
-        __syncwarp();
-        if (lane < nb)
-          bulk_g2s_hint(stage0 + s * C::kStage + (8 + lane) * C::kTile,
-                        vc + (size_t)blk * d.kv_block_stride + (size_t)cur.kvh * d.kv_head_stride, C::kTile, bar(ctl.full[s]), policy);
         if (b0 == 0) {
           scales_of(nxt, 0, ids_n, ks_n, vs_n);
           after = describe(__shfl_sync(0xffffffffu, claimed, 0));
@@ -342,21 +336,31 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
           mbar_arrive(bar(ctl.item_full[ic % kItemSlots]));
         }
       }
-    } else {
-      // drain: give copies already issued a bounded chance to land before shared memory goes away
-      for (uint32_t c = tc > C::kStages ? tc - C::kStages : 0; c < tc; ++c)
-        (void)mbar_wait_bounded(bar(ctl.full[c % C::kStages]), (c / C::kStages) & 1);
     }
   } else if (warp == C::kW0 + 1 || warp == C::kW0 + 2) {
-    // ================= K: 16-byte async copies, the chunk rows of the tile's blocks side by side =================
+    // ===== K: 16-byte async copies, the chunk rows of the tile's blocks side by side. V: bulk copies, by the first warp =====
     const uint8_t* kc = reinterpret_cast<const uint8_t*>(d.key_cache);
-    for (uint32_t tc = 0;; ++tc) {
+    const uint8_t* vc = reinterpret_cast<const uint8_t*>(d.value_cache);
+    const uint64_t policy = l2_policy_evict_first();
+    bool drain = true;
+    uint32_t tc = 0;
+    for (;; ++tc) {
       const int s = tc % C::kStages, r = tc % kDescSlots;
       if (!wait_or_abort(bar(ctl.desc_full[r]), (tc / kDescSlots) & 1, abort_flag, status)) break;
       const DecDesc& e = ctl.desc[r];
       const int nb = e.nb;
-      if (nb == 0) break;
+      if (nb == 0) {
+        drain = false;  // (the MMAs wait for all of it)
+        break;
+      }
       if (tc >= C::kStages && !wait_or_abort(bar(ctl.empty[s]), ((tc / C::kStages) & 1) ^ 1, abort_flag, status)) break;
+      if (warp == C::kW0 + 1) {
+        if (lane == 0) mbar_arrive_expect_tx(bar(ctl.full[s]), nb * C::kTile);
+        __syncwarp();
+        if (lane < nb)
+          bulk_g2s_hint(stage0 + s * C::kStage + (8 + lane) * C::kTile,
+                        vc + (size_t)e.blk[lane] * d.kv_block_stride + (size_t)e.kvh * d.kv_head_stride, C::kTile, bar(ctl.full[s]), policy);
+      }
       for (int j = warp - C::kW0 - 1; j < nb; j += 2) {
         const uint8_t* src = kc + (size_t)e.blk[j] * d.kv_block_stride + (size_t)e.kvh * d.kv_head_stride + lane * 16;
         const uint32_t dst = stage0 + s * C::kStage + (lane >> 4) * 2048 + j * 256 + (lane & 15) * 16;
@@ -366,6 +370,9 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
       cp_async_arrive_noinc(bar(ctl.full[s]));
     }
     cp_async_wait_all();
+    if (drain && warp == C::kW0 + 1)  // give copies already issued a bounded chance to land before shared memory goes away
+      for (uint32_t c = tc > C::kStages ? tc - C::kStages : 0; c < tc; ++c)
+        (void)mbar_wait_bounded(bar(ctl.full[c % C::kStages]), (c / C::kStages) & 1);
   } else if (warp == C::kW0 + 4) {
     // ================= query operands =================
     const uint8_t* qg = reinterpret_cast<const uint8_t*>(d.query);
@@ -516,6 +523,33 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
     uint32_t items = 0, x_use = 0;
 #pragma unroll
     for (int h = 0; h < N; ++h) { mul[h] = 0.f; ref[h] = -INFINITY; l[h] = 0.f; mx[h] = -INFINITY; }
+    // An item's partial: sums and exact maxima of the four warps, O from tensor memory. It waits for the product of the item's last
+    // tile, so it is put off until the next item's first weights are on their way (O and what is left of an item have two places).
+    bool pending = false;
+    uint32_t last_tc = 0;
+    auto epilogue = [&](uint32_t item, uint32_t tile) -> bool {
+      const int at = item & 1, row = ctl.left_row[g][at], head = ctl.left_head[g][at], part = ctl.left_part[g][at];
+      if (!wait_or_abort(bar(ctl.pv_done[tile & 1]), (tile >> 1) & 1, abort_flag, status)) return false;
+      tc_fence_after();
+      uint32_t o[kParts * N];
+      ld_cols<N>(tmem_o + at * C::kN + lane_base, o);
+      tmem_wait_ld();
+      tc_fence_before();
+#pragma unroll
+      for (int h = 0; h < N; ++h) {
+        if (h0 + h < hpi) {
+          const float m = max4(ctl.left_max[g][at][h]), ref_h = ctl.left_ref[g][at][h];
+          const float4 sums = ctl.left_sum[g][at][h];
+          const float sum = (sums.x + sums.y) + (sums.z + sums.w);
+          const float fix = ref_h == -INFINITY ? 0.f : fast_exp2(ref_h - m);
+          const float v = join_parts<N>(o, h);
+          const size_t slot = partial_slot(d, row, part, head + h0 + h);
+          if (r < D) d.acc[slot * D + r] = v * (fix * (1.f / 256));  // (2^-kTop)
+          if (r == 0) d.ml[slot] = make_float2(m, sum * fix);
+        }
+      }
+      return true;
+    };
     for (uint32_t tc = 0;; ++tc) {
       const int rr = tc % kDescSlots, s = tc % C::kStages, buf = tc & 1;
       if (!wait_or_abort(bar(ctl.desc_full[rr]), (tc / kDescSlots) & 1, abort_flag, status)) break;
@@ -630,41 +664,34 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
       fence_proxy_async_smem();
       tc_fence_before();
       mbar_arrive(bar(ctl.p_full[buf]));
+      if (pending) {
+        if (!epilogue(items - 2, tc - 1)) break;
+        pending = false;
+      }
       if (!last) continue;
-
-      // ---- the item's partial: sums and exact maxima from the four warps, O from tensor memory ----
+      // ---- what the item's epilogue needs is left in shared memory (this phase's exchange orders it) ----
+      const int at = (items - 1) & 1;
 #pragma unroll
       for (int h = 0; h < N; ++h) {
         mx[h] = warp_max(mx[h]);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+        if (r == 0) ctl.left_ref[g][at][h] = ref[h];
       }
-      leave(ctl.xmax[g][x_use & 1], mx, quarter, lane);
-      leave(ctl.xsum[g][x_use & 1], l, quarter, lane);
+      leave(ctl.left_max[g][at], mx, quarter, lane);
+      leave(ctl.left_sum[g][at], l, quarter, lane);
+      if (r == 0) {
+        ctl.left_row[g][at] = row;
+        ctl.left_head[g][at] = head;
+        ctl.left_part[g][at] = part;
+      }
+      pending = true;
+      last_tc = tc;
+    }
+    if (pending && *abort_flag == 0) {  // the last item's
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(ctl.exchange[g]));
-      if (!wait_or_abort(bar(ctl.exchange[g]), x_use & 1, abort_flag, status)) break;
-      const int eb = x_use & 1;
-      ++x_use;
-      if (!wait_or_abort(bar(ctl.pv_done[buf]), (tc >> 1) & 1, abort_flag, status)) break;
-      tc_fence_after();
-      uint32_t o[kParts * N];
-      ld_cols<N>(tmem_o + ((items - 1) & 1) * C::kN + lane_base, o);
-      tmem_wait_ld();
-      tc_fence_before();
-#pragma unroll
-      for (int h = 0; h < N; ++h) {
-        if (h0 + h < hpi) {
-          const float m = max4(ctl.xmax[g][eb][h]);
-          const float4 sums = ctl.xsum[g][eb][h];
-          const float sum = (sums.x + sums.y) + (sums.z + sums.w);
-          const float fix = ref[h] == -INFINITY ? 0.f : fast_exp2(ref[h] - m);
-          const float v = join_parts<N>(o, h);
-          const size_t slot = partial_slot(d, row, part, head + h0 + h);
-          if (r < D) d.acc[slot * D + r] = v * (fix * (1.f / 256));  // (2^-kTop)
-          if (r == 0) d.ml[slot] = make_float2(m, sum * fix);
-        }
-      }
+      if (wait_or_abort(bar(ctl.exchange[g]), x_use & 1, abort_flag, status)) (void)epilogue(items - 1, last_tc);
     }
   }
 
