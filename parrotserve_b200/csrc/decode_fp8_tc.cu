@@ -433,44 +433,56 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
     // ================= MMA issuer =================
     // S(t + 1) as soon as its tile is there, O(t) as soon as its weights are: whichever comes first.
     constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(C::kN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);  // fp32 += e4m3 . e4m3
-    const uint32_t q0 = smem_u32(smem + C::kOffQ), w0 = smem_u32(smem + C::kOffW);
+    // Descriptors: the operands' addresses (in sixteens of bytes) are added to words made once. (Made anew for every MMA by the one
+    // thread that issues them they cost more than the products: 1500 cycles a tile with their polls, ISSUE_NOW so.)
+    const uint64_t dk = smem_desc(stage0, 2048, 128, 0), dv = smem_desc(stage0 + 8 * C::kTile, C::kTile, 128, 0);
+    const uint64_t dq = smem_desc(smem_u32(smem + C::kOffQ), C::kN * 16, 128, 0), dw = smem_desc(smem_u32(smem + C::kOffW), C::kN * 16, 128, 0);
+    const uint32_t k_hi = (uint32_t)(dk >> 32), v_hi = (uint32_t)(dv >> 32), n_hi = (uint32_t)(dq >> 32);
+    const uint32_t k_lo = (uint32_t)dk, v_lo = (uint32_t)dv, q_lo = (uint32_t)dq, w_lo = (uint32_t)dw;
+    auto word = [](uint32_t hi, uint32_t lo) { return ((uint64_t)hi << 32) | lo; };
     uint32_t qk = 0, pv = 0;           // next tile of either product
     uint32_t qk_item = 0, pv_item = 0;  // items that have begun
+    int qk_nb = -1, pv_nb[2] = {0, 0};  // blocks of tile qk (-1: not seen yet), and of the tiles on their way
+    bool qk_first = false, qk_last = false, pv_first[2] = {false, false};
     bool ok = true, more = true;
     uint64_t t_start = 0;
     uint32_t spin = 0;
     while (ok && (more || pv < qk)) {
       bool progress = false;
       if (more && qk <= pv + 1) {
-        const int r = qk % kDescSlots, s = qk % C::kStages;
-        bool ready = mbar_test_wait(bar(ctl.desc_full[r]), (qk / kDescSlots) & 1);
-        ready = __all_sync(0xffffffffu, ready);
-        if (ready) {
-          const DecDesc& e = ctl.desc[r];
-          if (e.nb == 0) {
-            more = false;
+        const uint32_t r = qk % kDescSlots, s = qk % C::kStages;
+        if (qk_nb < 0) {
+          bool there = mbar_test_wait(bar(ctl.desc_full[r]), (qk / kDescSlots) & 1);
+          there = __all_sync(0xffffffffu, there);
+          if (there) {
+            const DecDesc& e = ctl.desc[r];
+            qk_nb = e.nb; qk_first = e.first; qk_last = e.last;
+            if (qk_nb == 0) more = false;
             progress = true;
-          } else {
-            const uint32_t item = qk_item + (e.first ? 1 : 0) - 1;
-            ready = mbar_test_wait(bar(ctl.full[s]), (qk / C::kStages) & 1) && mbar_test_wait(bar(ctl.q_full[item & 1]), (item >> 1) & 1);
-            ready = __all_sync(0xffffffffu, ready);
-            if (ready) {
-              fence_proxy_async_smem();  // K was written by per-thread async copies
-              tc_fence_after();
-              if (lane == 0) {
-                const uint32_t k0 = stage0 + s * C::kStage, b0 = q0 + (item & 1) * C::kQ;
+          }
+        }
+        if (qk_nb > 0) {
+          const uint32_t item = qk_item + (qk_first ? 1 : 0) - 1;
+          bool ready = mbar_test_wait(bar(ctl.full[s]), (qk / C::kStages) & 1);
+          if (qk_first) ready = ready && mbar_test_wait(bar(ctl.q_full[item & 1]), (item >> 1) & 1);
+          ready = __all_sync(0xffffffffu, ready);
+          if (ready) {
+            fence_proxy_async_smem();  // K was written by per-thread async copies
+            tc_fence_after();
+            if (lane == 0) {
+              const uint32_t a = k_lo + s * (C::kStage >> 4), b = q_lo + (item & 1) * (C::kQ >> 4), to = tmem_s + (qk & 1) * C::kN;
 #pragma unroll
-                for (int kk = 0; kk < D / 32; ++kk)  // 32 of d: two 16-byte chunks
-                  mma_f8(tmem_s + (qk & 1) * C::kN, smem_desc(k0 + kk * 2 * 2048, 2048, 128, 0),
-                         smem_desc(b0 + kk * 2 * C::kN * 16, C::kN * 16, 128, 0), kIdesc, kk > 0 ? 1u : 0u);
-                mma_commit(bar(ctl.s_full[qk & 1]));
-                if (e.last) mma_commit(bar(ctl.q_empty[item & 1]));
-              }
-              __syncwarp();
-              qk_item = item + 1;
-              ++qk;
-              progress = true;
+              for (int kk = 0; kk < D / 32; ++kk)  // 32 of d: two 16-byte chunks
+                mma_f8(to, word(k_hi, a + kk * (2 * 2048 >> 4)), word(n_hi, b + kk * 2 * C::kN), kIdesc, kk > 0 ? 1u : 0u);
+              mma_commit(bar(ctl.s_full[qk & 1]));
+              if (qk_last) mma_commit(bar(ctl.q_empty[item & 1]));
             }
+            __syncwarp();
+            if (qk & 1) { pv_nb[1] = qk_nb; pv_first[1] = qk_first; } else { pv_nb[0] = qk_nb; pv_first[0] = qk_first; }
+            qk_item = item + 1;
+            ++qk;
+            qk_nb = -1;
+            progress = true;
           }
         }
       }
@@ -479,20 +491,21 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
         ready = __all_sync(0xffffffffu, ready);
         if (ready) {
           tc_fence_after();
-          const int r = pv % kDescSlots, s = pv % C::kStages;
-          const DecDesc& e = ctl.desc[r];
-          pv_item += e.first ? 1 : 0;
+          const uint32_t r = pv % kDescSlots, s = pv % C::kStages;
+          const int nb = (pv & 1) ? pv_nb[1] : pv_nb[0];
+          const bool first = (pv & 1) ? pv_first[1] : pv_first[0];
+          pv_item += first ? 1 : 0;
           if (lane == 0) {
-            const uint32_t v0 = stage0 + s * C::kStage + 8 * C::kTile, b0 = w0 + (pv & 1) * C::kW;
-            const int steps = (e.nb + 1) / 2;  // 32 tokens: two blocks (the softmax threads have cleared what is missing)
-            for (int kk = 0; kk < steps; ++kk)
-              mma_f8(tmem_o + ((pv_item - 1) & 1) * C::kN, smem_desc(v0 + kk * 2 * C::kTile, C::kTile, 128, 0),
-                     smem_desc(b0 + kk * 2 * C::kN * 16, C::kN * 16, 128, 0), kIdesc, (kk > 0 || !e.first) ? 1u : 0u);
+            const uint32_t a = v_lo + s * (C::kStage >> 4), b = w_lo + (pv & 1) * (C::kW >> 4), to = tmem_o + ((pv_item - 1) & 1) * C::kN;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)  // 32 tokens: two blocks (the softmax threads have cleared what is missing)
+              if (2 * kk < nb)
+                mma_f8(to, word(v_hi, a + kk * (2 * C::kTile >> 4)), word(n_hi, b + kk * 2 * C::kN), kIdesc, (kk > 0 || !first) ? 1u : 0u);
             mma_commit(bar(ctl.empty[s]));
             mma_commit(bar(ctl.pv_done[pv & 1]));
+            mbar_arrive(bar(ctl.desc_empty[r]));
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(ctl.desc_empty[r]));
           ++pv;
           progress = true;
         }
