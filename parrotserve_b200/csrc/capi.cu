@@ -309,18 +309,19 @@ int run_stages(const pb_attn_params* p, const AttnDev& d_in, cudaStream_t s) {
 }
 
 // ---- the same over the 8-bit cache ----
-// Blocks per item of the single-query kernel. On tcgen05 a tile is eight blocks and an item costs about a tile beside them, so
-// items are as long as leaves two for every CTA of the chip, if the rows are half full on average. In us, with chunks of 8 / 16 /
-// 32 / 128 blocks: 64 rows of 512 tokens, 32 heads 65 / 53 / 52 / 52; 256 of 1024 431 / 346 / 341 / 326; 128 of 1024, 32 heads over 8
-// 87 / 74 / 67 / 71; 3 of 300 9.4 / 9.9 / 11.6 / 11.6. (The mma.sync kernel keeps the rule of the 16-bit caches.)
+// Blocks per item of the single-query kernel. On tcgen05 a tile is eight blocks and an item costs most of a tile beside them, so
+// items are as long as leaves two for every CTA of the chip, up to 64 blocks (longer ones gain nothing and end unevenly). In us,
+// with chunks of 8 / 16 / 32 / 64 / 128 blocks: 64 rows of 512 tokens, 32 heads 56 / 51 / 51 / 51 / 51; 256 of 1024 367 / 326 / 318 / 316 /
+// 317; 128 of 16 to 2048 tokens, 32 heads over 8 107 / 89 / 82 / 81 / 84; one of 100003 tokens, 64 heads over 8 149 / 99 / 84 / 74 / 79; 3 of
+// 300, 32 heads 9.2 / 9.7 / 11.1 / 11.1 / 11.1. (The mma.sync kernel keeps the rule of the 16-bit caches.)
 pb_attn_params with_fp8_chunks(const pb_attn_params* p) {
   pb_attn_params q = *p;
   if (q.suffix_chunk_blocks <= 0 && decode_fp8_supported(q.dtype, q.head_size, q.block_size) && q.num_heads > 0 && q.num_rows > 0) {
     const int share = heads_per_item(&q);
     const long long ctas = (long long)sm_count() * (share > 1 ? 2 : 3);
-    const long long blocks = (long long)q.num_rows * (q.num_heads / share) * q.suffix_table_stride / 2;
+    const long long blocks = (long long)q.num_rows * (q.num_heads / share) * q.suffix_table_stride;
     const int cs = pow2_floor(blocks / (2 * ctas) > 0 ? blocks / (2 * ctas) : 1);
-    q.suffix_chunk_blocks = cs < 8 ? 8 : cs > 128 ? 128 : cs;
+    q.suffix_chunk_blocks = cs < 8 ? 8 : cs > 64 ? 64 : cs;
   }
   return q;
 }

@@ -57,11 +57,12 @@ struct DecCfg {
   static constexpr int kW0 = 4 * kGroups;             // the first warp behind them
   static constexpr int kThreads = 32 * (kW0 + 5);
   static constexpr int kCtas = HMAX > 1 ? 2 : 3;      // per SM
-  static constexpr int kStages = HMAX == 1 ? 2 * 128 / D : HMAX == 4 ? 3 * 128 / D : D == 128 ? 2 : D == 96 ? 3 : 5;
+  static constexpr int kStages = (HMAX == 1 ? 2 : 3) * 128 / D;
+  static constexpr int kQSlots = HMAX > 4 ? 1 : 2;    // query operands: of the item at work, and of the next if there is room
   static constexpr int kQ = kN * D, kW = kN * 128;    // operands of one item / one tile
   // rows of V beyond D (the MMA always has 128) are read from what lies behind the tile: kPad bytes behind the last stage
   static constexpr int kPad = (128 - D) * 16;
-  static constexpr int kOffW = kStages * kStage + kPad, kOffQ = kOffW + 2 * kW, kOffCtl = kOffQ + 2 * kQ;
+  static constexpr int kOffW = kStages * kStage + kPad, kOffQ = kOffW + 2 * kW, kOffCtl = kOffQ + kQSlots * kQ;
   static constexpr int kTmem = kN == 32 ? 128 : 64;   // S, S, O, O
 };
 
@@ -382,13 +383,13 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(ctl.item_empty[ic % kItemSlots]));
       if (row < 0) break;
-      const int slot = ic & 1;
+      const int slot = ic % C::kQSlots;
       uint2 raw[HMAX];
 #pragma unroll
       for (int h = 0; h < HMAX; ++h)
         raw[h] = (h < hpi && lane < D / 4) ? *reinterpret_cast<const uint2*>(qg + ((size_t)row * d.q_stride + (size_t)(head + h) * D + 4 * lane) * 2)
                                            : make_uint2(0u, 0u);
-      if (ic >= 2 && !wait_or_abort(bar(ctl.q_empty[slot]), ((ic >> 1) & 1) ^ 1, abort_flag, status)) break;
+      if (ic >= C::kQSlots && !wait_or_abort(bar(ctl.q_empty[slot]), ((ic / C::kQSlots) & 1) ^ 1, abort_flag, status)) break;
       uint8_t* qop = smem + C::kOffQ + slot * C::kQ;
 #pragma unroll
       for (int h = 0; h < HMAX; ++h) {
@@ -464,18 +465,18 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
         if (qk_nb > 0) {
           const uint32_t item = qk_item + (qk_first ? 1 : 0) - 1;
           bool ready = mbar_test_wait(bar(ctl.full[s]), (qk / C::kStages) & 1);
-          if (qk_first) ready = ready && mbar_test_wait(bar(ctl.q_full[item & 1]), (item >> 1) & 1);
+          if (qk_first) ready = ready && mbar_test_wait(bar(ctl.q_full[item % C::kQSlots]), (item / C::kQSlots) & 1);
           ready = __all_sync(0xffffffffu, ready);
           if (ready) {
             fence_proxy_async_smem();  // K was written by per-thread async copies
             tc_fence_after();
             if (lane == 0) {
-              const uint32_t a = k_lo + s * (C::kStage >> 4), b = q_lo + (item & 1) * (C::kQ >> 4), to = tmem_s + (qk & 1) * C::kN;
+              const uint32_t a = k_lo + s * (C::kStage >> 4), b = q_lo + (item % C::kQSlots) * (C::kQ >> 4), to = tmem_s + (qk & 1) * C::kN;
 #pragma unroll
               for (int kk = 0; kk < D / 32; ++kk)  // 32 of d: two 16-byte chunks
                 mma_f8(to, word(k_hi, a + kk * (2 * 2048 >> 4)), word(n_hi, b + kk * 2 * C::kN), kIdesc, kk > 0 ? 1u : 0u);
               mma_commit(bar(ctl.s_full[qk & 1]));
-              if (qk_last) mma_commit(bar(ctl.q_empty[item & 1]));
+              if (qk_last) mma_commit(bar(ctl.q_empty[item % C::kQSlots]));
             }
             __syncwarp();
             if (qk & 1) { pv_nb[1] = qk_nb; pv_first[1] = qk_first; } else { pv_nb[0] = qk_nb; pv_first[0] = qk_first; }
@@ -572,8 +573,8 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
       if (nb == 0) break;
       const float ks = e.ks[blk_of], lv = e.lv[blk_of];
       if (first) {
-        const int slot = items & 1;
-        if (!wait_or_abort(bar(ctl.q_full[slot]), (items >> 1) & 1, abort_flag, status)) break;
+        const int slot = items % C::kQSlots;
+        if (!wait_or_abort(bar(ctl.q_full[slot]), (items / C::kQSlots) & 1, abort_flag, status)) break;
 #pragma unroll
         for (int h = 0; h < N; ++h) { mul[h] = ctl.mul[slot][h0 + h]; ref[h] = -INFINITY; l[h] = 0.f; mx[h] = -INFINITY; }
         __syncwarp();
