@@ -31,6 +31,7 @@ namespace {
 
 using namespace dense;
 using fp8::kMinLv;
+using fp8::warp_max;
 
 constexpr int kDescSlots = 8, kItemSlots = 4;  // (how far the lister runs ahead: it waits for three loads in a row per item)
 constexpr int kParts = 4;                  // the MMA takes sixteen columns or none: four parts cost what three do
@@ -137,12 +138,6 @@ __device__ __forceinline__ void parts_of_two(float x, float y, uint32_t (&p)[kPa
   const uint32_t b = fp8::to_half2(p[2]);
   r = __hmul2(__hsub2(r, *reinterpret_cast<const __half2*>(&b)), __float2half2_rn(16.f));
   p[3] = fp8::pack2(r);
-}
-// Maximum over a warp (NaN counts as nothing, like fmaxf).
-__device__ __forceinline__ float warp_max(float v) {
-  float m;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
-  return m;
 }
 __device__ __forceinline__ float max4(float4 v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
 // Lane h < N leaves v[h] (the same in all lanes) as warp w's number of head h.

@@ -28,6 +28,7 @@ namespace {
 
 using namespace dense;
 using fp8::kMinLv;
+using fp8::warp_max;
 
 constexpr float kShift = 7.f;                            // w <= 2^(kTau + kShift) = 2^15
 constexpr int kCodeBytes = kBlkBytes / 2;                // one K or V tile of a (block, head): 2 KiB
@@ -97,47 +98,56 @@ template <typename T> struct Layout {
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
-// ---- query rows as sums of e4m3 parts: a warp per (row, head), four elements a lane ----
+// ---- query rows as sums of e4m3 parts: a CTA per row and 32 heads, a warp four heads, a lane four elements of each ----
+// (A warp per (row, head) had too little on its way to memory: 10714 rows x 32 heads 72 us, 48 so.)
+constexpr int kPartsHeads = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) query_parts_kernel(const AttnDev d) {
   pdl_wait();  // the workspace may still be the kernel's before this one
   pdl_trigger();
   const int lane = threadIdx.x & 31;
-  const long long idx = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (idx >= (long long)d.num_rows * d.num_heads) return;
-  const int row = (int)(idx / d.num_heads), head = (int)(idx - (long long)row * d.num_heads);
-  const uint2 raw = *reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(d.query) + (size_t)row * d.q_stride + (size_t)head * kD + 4 * lane);
-  float f[4];
-  if constexpr (Pack<T>::kBf16) {
-    f[0] = __uint_as_float(raw.x << 16); f[1] = __uint_as_float(raw.x & 0xffff0000u);
-    f[2] = __uint_as_float(raw.y << 16); f[3] = __uint_as_float(raw.y & 0xffff0000u);
-  } else {
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+  const int row = blockIdx.x, h0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * kPartsHeads;
+  uint2 in[kPartsHeads];
+#pragma unroll
+  for (int k = 0; k < kPartsHeads; ++k)
+    if (h0 + k < d.num_heads)
+      in[k] = *reinterpret_cast<const uint2*>(reinterpret_cast<const T*>(d.query) + (size_t)row * d.q_stride + (size_t)(h0 + k) * kD + 4 * lane);
+#pragma unroll
+  for (int k = 0; k < kPartsHeads; ++k) {
+    const int head = h0 + k;
+    if (head >= d.num_heads) break;
+    const uint2 raw = in[k];
+    float f[4];
+    if constexpr (Pack<T>::kBf16) {
+      f[0] = __uint_as_float(raw.x << 16); f[1] = __uint_as_float(raw.x & 0xffff0000u);
+      f[2] = __uint_as_float(raw.y << 16); f[3] = __uint_as_float(raw.y & 0xffff0000u);
+    } else {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+      f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+    }
+    float top = 0.f;
+    bool odd = false;  // NaN or an infinity: the parts could not say so
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      top = fmaxf(top, fabsf(f[i]));
+      odd = odd || !(fabsf(f[i]) <= 3.402823466e38f);
+    }
+    top = warp_max(top);
+    odd = __any_sync(0xffffffffu, odd);
+    const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
+    const float up = __uint_as_float((uint32_t)(261 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] *= up;
+#pragma unroll
+    for (int p = 0; p < QParts<T>::kNum; ++p) {
+      const uint32_t lo = fp8::pack2(f[0], f[1]), hi = fp8::pack2(f[2], f[3]);
+      const float2 a = fp8::to_float2(lo), b = fp8::to_float2(hi);
+      f[0] -= a.x; f[1] -= a.y; f[2] -= b.x; f[3] -= b.y;
+      *reinterpret_cast<uint32_t*>(d.q_parts + (((size_t)p * d.num_heads + head) * d.num_rows + row) * kD + 4 * lane) = lo | (hi << 16);
+    }
+    if (lane == 0)
+      d.q_mul[(size_t)head * d.num_rows + row] = odd ? __int_as_float(0x7fc00000) : d.scale_log2e * __uint_as_float((uint32_t)(e - 7) << 23);
   }
-  float top = 0.f;
-  bool odd = false;  // NaN or an infinity: the parts could not say so
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    top = fmaxf(top, fabsf(f[i]));
-    odd = odd || !(fabsf(f[i]) <= 3.402823466e38f);
-  }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  odd = __any_sync(0xffffffffu, odd);
-  const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
-  const float up = __uint_as_float((uint32_t)(261 - e) << 23);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] *= up;
-#pragma unroll
-  for (int p = 0; p < QParts<T>::kNum; ++p) {
-    const uint32_t lo = fp8::pack2(f[0], f[1]), hi = fp8::pack2(f[2], f[3]);
-    const float2 a = fp8::to_float2(lo), b = fp8::to_float2(hi);
-    f[0] -= a.x; f[1] -= a.y; f[2] -= b.x; f[3] -= b.y;
-    *reinterpret_cast<uint32_t*>(d.q_parts + (((size_t)p * d.num_heads + head) * d.num_rows + row) * kD + 4 * lane) = lo | (hi << 16);
-  }
-  if (lane == 0)
-    d.q_mul[(size_t)head * d.num_rows + row] = odd ? __int_as_float(0x7fc00000) : d.scale_log2e * __uint_as_float((uint32_t)(e - 7) << 23);
 }
 
 // The warp that lists the tiles: block ids, scales and extents of every kv tile of this CTA, as far ahead as the ring allows.
@@ -428,7 +438,15 @@ struct RowState {
   float m_run, l_run, m_true;
 };
 
-template <typename T>
+// A lone row tile of a shared prefix is worked on by both softmax groups and issuers: group x takes its kv tiles x, x + 2, ... with
+// Q_0, S_x and O_x, and group 0 joins the two O in the epilogue. By one group alone each tile waits for the one before it: S,
+// softmax, P.V, 3.4 us against 2.4 (64 rows over 65536 tokens, 32 heads: 286 us). The last row tiles of prefills stay with group 0:
+// they take what a pair takes, and the shares of the CTAs, which count a tile of either as one, stay even (16 prefills of 256 to
+// 1024 tokens and 240 decodes over 2048 tokens: 1160 us with both groups, 1015 with one).
+// (kSplit: the call has no prefills.)
+__device__ __forceinline__ int first_tile(bool pair, bool split, int x, int n) { return (pair || x == 0) ? 0 : split ? 1 : n; }
+
+template <typename T, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
 dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap amap,
                  const __grid_constant__ CUtensorMap omap) {
@@ -516,9 +534,8 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
     while (ok && walk.next(sg)) {
       const int n = sg.t1 - sg.t0;
       const bool pair = sg.it.nrows > 128;
-      // A lone row tile is worked on by both groups: group x takes its kv tiles x, x + 2, ... with Q_0, S_x and O_x, and group 0
-      // joins the two O in the epilogue. (By one group alone each tile waits for the one before it: S, softmax, P.V, 3.3 us.)
-      const int first = pair ? 0 : x, step = pair ? 1 : 2;
+      const bool split = kSplit && !pair;
+      const int first = first_tile(pair, split, x, n), step = split ? 2 : 1;
       const uint64_t bq = pair ? desc_q : desc_q0;
       // S_x = Q_x . K(i)^T (the caller has seen K(i) land); lane 0 only
       auto qk_mmas = [&](int i) {
@@ -531,13 +548,13 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
 #pragma unroll
           for (int kk = 0; kk < kD / 32; ++kk)
             mma_f8(tmem_s, bq + ((p * kPartBytes + kk * 32) >> 4), bk + ((kk * 2 * 2048) >> 4), idesc, (p | kk) ? 1u : 0u);
-        mma_commit(bar(kBarS + x));
       };
       auto qk_release = [&](int i) {
+        mma_commit(bar(kBarS + x));
         mma_commit(bar(kBarEmptyK + ((tc + i) & 1)));
         if (i + step >= n) {  // this issuer's last Q.K^T of the segment
           mma_commit(bar(kBarQFree + (pair ? x : 0)));
-          if (x == 0 && pair) mma_commit(bar(kBarQFree));  // (the other issuer does not read Q_0)
+          if (x == 0 && !split) mma_commit(bar(kBarQFree));  // (the other issuer does not read Q_0)
         }
       };
       // A wait names its phase by parity alone, so nobody may be two phases away from what it waits for. Ring slots take a release
@@ -554,9 +571,15 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         if (lane == 0) mbar_arrive(bar(kBarEmptyV + ((tc + i) & 1)));
         return true;
       };
+      if (!split && !pair && x == 1) {  // nothing for this issuer but its releases
+        for (int i = 0; i < n && ok; ++i) ok = pass_k(i) && pass_v(i);
+        tc += n;
+        ++seg;
+        continue;
+      }
       if (!wait_or_abort(bar(kBarQ + (pair ? x : 0)), (pair && x == 1 ? pairs : seg) & 1, abort_flag, status)) { ok = false; break; }
-      if (first >= n && lane == 0) mbar_arrive(bar(kBarQFree));  // (a lone row tile of one kv tile: nothing for this issuer)
-      if (first == 1 && !pass_k(0)) { ok = false; break; }
+      if (split && first >= n && lane == 0) mbar_arrive(bar(kBarQFree));  // (a lone row tile of one kv tile: nothing for this issuer)
+      if (split && x == 1 && !pass_k(0)) { ok = false; break; }
       if (first < n) {
         if (!full_k(first)) { ok = false; break; }
         fence_proxy_async_smem();  // K was written by per-thread async copies (generic proxy)
@@ -567,7 +590,7 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         }
         __syncwarp();
       }
-      if (first == 1 && !pass_v(0)) { ok = false; break; }
+      if (split && x == 1 && !pass_v(0)) { ok = false; break; }
       for (int i = first; i < n; i += step, ++tcx) {
         const uint32_t c = tc + i;
         const int s = c & 1;
@@ -575,7 +598,7 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         // what arrives early first: V(i), the next K; then P_x(i), which the chain hangs on, and the drained O_x (behind P_x: an
         // issuer without a tile in the last segment knows by it that the segment before that is over)
         if (!full_v(i)) { ok = false; break; }
-        if (pair && more && !full_k(i + 1)) { ok = false; break; }
+        if (!split && more && !full_k(i + 1)) { ok = false; break; }
         fence_proxy_async_smem();
         if (!wait_or_abort(bar(kBarP + x), tcx & 1, abort_flag, status)) { ok = false; break; }
         if (i == first && seg > 0 && !wait_or_abort(bar(kBarODrained + x), (seg - 1) & 1, abort_flag, status)) { ok = false; break; }
@@ -588,18 +611,16 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
 #pragma unroll
           for (int j = 0; j < kTileBlocks; ++j)
             if (j < nb) mma_f16_ts(tmem_o, tmem_s + j * 8, bv + j * (kBlkBytes >> 4), kIdescPV, (i > first || j > 0) ? 1u : 0u);
-          if (pair) {
-            if (more) qk_mmas(i + 1);  // behind P_x.V(i) in the pipe: it overwrites S_x / P_x
-            mbar_arrive(bar(kBarTurn + x));
-          }
+          if (!split && more) qk_mmas(i + 1);  // behind P_x.V(i) in the pipe: it overwrites S_x / P_x
+          if (pair) mbar_arrive(bar(kBarTurn + x));
           // (before the next S is announced: a softmax thread waits for this phase only with its last tile)
           mma_commit(bar(kBarPV + x));
+          if (!split && more) qk_release(i + 1);
           mma_commit(bar(kBarEmptyV + s));
-          if (pair && more) qk_release(i + 1);
         }
         if (pair) ++turns;
         __syncwarp();
-        if (!pair) {
+        if (split) {
           // the tile behind it is the other issuer's; the K of the next one of this issuer comes into the slot of this tile
           if (i + 1 < n && !pass_k(i + 1)) { ok = false; break; }
           if (more) {
@@ -650,7 +671,8 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
     while (ok && walk.next(sg)) {
       const DnItem& it = sg.it;
       const bool pair = it.nrows > 128;
-      const int first = sg.t0 + (pair ? 0 : x), step = pair ? 1 : 2;
+      const bool split = kSplit && !pair;
+      const int first = sg.t0 + first_tile(pair, split, x, sg.t1 - sg.t0), step = split ? 2 : 1;
       const int qrow = (pair ? x * 128 : 0) + r;  // row inside the item
       RowState st = {-INFINITY, 0.f, -INFINITY};
       const float mul = d.q_mul[(size_t)sg.head * d.num_rows + min(it.row0 + qrow, d.num_rows - 1)];
@@ -703,7 +725,7 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
       if (sg.t1 > first && !wait_or_abort(bar(kBarPV + x), (tcx - 1) & 1, abort_flag, status)) { ok = false; break; }
       tc_fence_after();
       if (!pair) {
-        const bool both = sg.t1 - sg.t0 > 1;
+        const bool both = split && sg.t1 - sg.t0 > 1;
         if (x == 1) {
           // hand over: O_1 stays where it is, lane for lane beside O_0. The last hand-over has been read by now.
           if (seg > 0 && !wait_or_abort(bar(kBarODrained + 1), (seg - 1) & 1, abort_flag, status)) { ok = false; break; }
@@ -849,15 +871,21 @@ template <auto kKernel> cudaError_t check_register_shares() {
   return verdict;
 }
 
-template <typename T>
-cudaError_t launch_t(const AttnDev& d, const CUtensorMap& pmap, const CUtensorMap& amap, const CUtensorMap& omap, cudaStream_t s) {
-  auto kfn = dense_fp8_kernel<T>;
+template <typename T, bool kSplit>
+cudaError_t launch_dense(const AttnDev& d, const CUtensorMap& pmap, const CUtensorMap& amap, const CUtensorMap& omap, cudaStream_t s) {
+  auto kfn = dense_fp8_kernel<T, kSplit>;
   cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T>::kSmemBytes);
-  if (e == cudaSuccess) e = check_register_shares<dense_fp8_kernel<T>>();
-  const long long pairs = (long long)d.num_rows * d.num_heads;
-  if (e == cudaSuccess) e = launch_kernel(query_parts_kernel<T>, dim3((unsigned)((pairs + 7) / 8)), 256, 0, s, true, d);
+  if (e == cudaSuccess) e = check_register_shares<dense_fp8_kernel<T, kSplit>>();
   if (e != cudaSuccess) return e;
   return launch_kernel(kfn, d.num_sms, kThreads, Layout<T>::kSmemBytes, s, true, d, pmap, amap, omap);
+}
+
+template <typename T>
+cudaError_t launch_t(const AttnDev& d, const CUtensorMap& pmap, const CUtensorMap& amap, const CUtensorMap& omap, cudaStream_t s) {
+  const dim3 grid((unsigned)d.num_rows, (unsigned)((d.num_heads + 8 * kPartsHeads - 1) / (8 * kPartsHeads)));
+  const cudaError_t e = launch_kernel(query_parts_kernel<T>, grid, 256, 0, s, true, d);
+  if (e != cudaSuccess) return e;
+  return d.num_segments == 0 ? launch_dense<T, true>(d, pmap, amap, omap, s) : launch_dense<T, false>(d, pmap, amap, omap, s);
 }
 
 }  // namespace

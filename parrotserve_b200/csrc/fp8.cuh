@@ -39,5 +39,12 @@ __device__ __forceinline__ float scale_for(float top) {
   return __uint_as_float((uint32_t)(e < 1 ? 1 : e) << 23);
 }
 
+// Maximum over a warp (NaN counts as nothing, like fmaxf).
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
 }  // namespace fp8
 }  // namespace pb
