@@ -280,57 +280,77 @@ __device__ __forceinline__ void fill_tile(const uint8_t* rows, size_t row_bytes,
   if (lane == 0 && now == held && (mask & 1u)) *scale = now;  // (0: what the block's last owner left is void)
 }
 
-// One token alone in its block: lanes 0-15 take its K row, 16-31 its V row. False, and nothing written, if a scale has to
-// grow under other tokens.
+// One token alone in its block, under kRowHeads heads from h0 (nh of them are there): lanes 0-15 take its K rows, 16-31 its V rows.
+// Returns the tiles that are left to fill_tile, two bits a head: those of heads where a scale has to grow under other tokens, or with a NaN or an
+// infinity.
+constexpr int kRowHeads = 4;
 template <typename T, int D, int B>
-__device__ __forceinline__ bool fill_row(const Fp8Rows& a, long long blk, int h, int m, int off, int lane) {
+__device__ __forceinline__ uint32_t fill_rows(const Fp8Rows& a, long long blk, int h0, int nh, int m, int off, int lane) {
   constexpr int kPer = (D / 8 + 15) / 16;
   const int v = lane >> 4, l = lane & 15;
-  const uint8_t* row = (v ? a.value : a.key) + ((size_t)m * (v ? a.value_stride : a.key_stride) + (size_t)h * D) * sizeof(T);
-  uint8_t* tile = (v ? a.vcache : a.kcache) + (size_t)blk * a.kbs + (size_t)h * a.khs;
-  float* scale = (v ? a.vscale : a.kscale) + (size_t)blk * a.sbs + (size_t)h * a.shs;
-  Raw8<T> raw[kPer];
-  uint32_t bits = 0;
+  const uint8_t* row = (v ? a.value : a.key) + ((size_t)m * (v ? a.value_stride : a.key_stride) + (size_t)h0 * D) * sizeof(T);
+  uint8_t* tile = (v ? a.vcache : a.kcache) + (size_t)blk * a.kbs + (size_t)h0 * a.khs;
+  float* scale = (v ? a.vscale : a.kscale) + (size_t)blk * a.sbs + (size_t)h0 * a.shs;
+  Raw8<T> raw[kRowHeads][kPer];
+  float held[kRowHeads];
 #pragma unroll
-  for (int p = 0; p < kPer; ++p) {
-    raw[p].clear();
-    if (p * 16 + l < D / 8) raw[p].load(row + (p * 16 + l) * 8 * sizeof(T));
-  }
-  const float held = off == 0 ? 0.f : *scale;
+  for (int h = 0; h < kRowHeads; ++h) {
+    held[h] = (h < nh && off != 0) ? scale[(size_t)h * a.shs] : 0.f;
 #pragma unroll
-  for (int p = 0; p < kPer; ++p) raw[p].top_bits(bits);
-  float top = top_of<T>(bits);
-#pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) top = __uint_as_float(max(__float_as_uint(top), __shfl_xor_sync(0xffffffffu, __float_as_uint(top), o)));
-  const float now = fmaxf(held, fp8::scale_for(top));
-  if (__any_sync(0xffffffffu, !is_finite(top) || (held > 0.f && now > held))) return false;
-  const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
-#pragma unroll
-  for (int p = 0; p < kPer; ++p) {
-    const int c = p * 16 + l;
-    if (c >= D / 8) continue;
-    float f[8];
-    raw[p].floats(f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = __fmul_rn(f[k], inv);
-    const uint2 w = make_uint2(fp8::pack4(f[0], f[1], f[2], f[3]), fp8::pack4(f[4], f[5], f[6], f[7]));
-    if (v == 0) {
-      *reinterpret_cast<uint2*>(tile + ((c >> 1) * B + off) * 16 + 8 * (c & 1)) = w;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) tile[(c * 8 + k) * B + off] = (uint8_t)((k < 4 ? w.x : w.y) >> (8 * (k & 3)));
+    for (int p = 0; p < kPer; ++p) {
+      raw[h][p].clear();
+      if (h < nh && p * 16 + l < D / 8) raw[h][p].load(row + (h * D + (p * 16 + l) * 8) * sizeof(T));
     }
   }
-  if (l == 0) *scale = now;  // (behind the shuffles: every lane has read it)
-  return true;
+  uint32_t left = 0;
+#pragma unroll
+  for (int h = 0; h < kRowHeads; ++h) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) raw[h][p].top_bits(bits);
+    float top = top_of<T>(bits);
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) top = __uint_as_float(max(__float_as_uint(top), __shfl_xor_sync(0xffffffffu, __float_as_uint(top), o)));
+    const float now = fmaxf(held[h], fp8::scale_for(top));
+    if (__any_sync(0xffffffffu, !is_finite(top) || (held[h] > 0.f && now > held[h]))) {
+      left |= 3u << (2 * h);
+      continue;
+    }
+    if (h >= nh) continue;
+    const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      const int c = p * 16 + l;
+      if (c >= D / 8) continue;
+      float f[8];
+      raw[h][p].floats(f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = __fmul_rn(f[k], inv);
+      const uint2 w = make_uint2(fp8::pack4(f[0], f[1], f[2], f[3]), fp8::pack4(f[4], f[5], f[6], f[7]));
+      uint8_t* t = tile + (size_t)h * a.khs;
+      if (v == 0) {
+        *reinterpret_cast<uint2*>(t + ((c >> 1) * B + off) * 16 + 8 * (c & 1)) = w;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[(c * 8 + k) * B + off] = (uint8_t)((k < 4 ? w.x : w.y) >> (8 * (k & 3)));
+      }
+    }
+    if (l == 0) scale[(size_t)h * a.shs] = now;  // (behind the shuffles: every lane has read it)
+  }
+  return left;
 }
+
+// CTAs an SM: two where the rows of a tile take 64 registers, three where they take fewer or are read twice. (Left to itself the
+// compiler takes up to 210 registers: 930 rows of fp32, heads of 80, blocks of 32, 41 us.)
+template <typename T, int D, int B> constexpr int kRowWords = (B / 16) * ((D / 8 + 7) / 8) * 16 * (int)sizeof(T) / 2;
+template <typename T, int D, int B> constexpr int kFillCtas = kRowWords<T, D, B> > 32 && kRowWords<T, D, B> <= 64 ? 2 : 3;
 
 // A CTA: 16 consecutive entries of slot_mapping, the blocks whose first token is among them, and one head or a few. A warp
 // takes one (block, head) at a time.
 template <typename T, int D, int B>
-__global__ void __launch_bounds__(kWarps * 32) fp8_fill_kernel(const Fp8Rows a, const int heads_per_cta) {
+__global__ void __launch_bounds__(kWarps * 32, kFillCtas<T, D, B>) fp8_fill_kernel(const Fp8Rows a, const int heads_per_cta) {
   __shared__ int member[16][B];
-  __shared__ int first[16], own[16], n_own;
+  __shared__ int first[16], many[16], lone[16], n_many, n_lone;  // (the blocks of this window with several tokens, and with one)
   __shared__ long long block_of[16];
   pdl_wait();
   pdl_trigger();
@@ -376,33 +396,54 @@ __global__ void __launch_bounds__(kWarps * 32) fp8_fill_kernel(const Fp8Rows a, 
   __syncthreads();
   if (warp == 0) {
     const bool mine = lane < 16 && block_of[lane & 15] >= 0 && first[lane & 15] >= t0 && first[lane & 15] < t0 + 16;
-    const unsigned all = __ballot_sync(0xffffffffu, mine);
-    if (mine) own[__popc(all & ((1u << lane) - 1u))] = lane;
-    if (lane == 0) n_own = __popc(all);
+    int count = 0;
+    if (mine)
+      for (int off = 0; off < B; ++off) count += member[lane][off] >= 0;
+    const unsigned ones = __ballot_sync(0xffffffffu, mine && count == 1), others = __ballot_sync(0xffffffffu, mine && count != 1);
+    const unsigned before = (1u << lane) - 1u;
+    if (mine && count == 1) lone[__popc(ones & before)] = lane;
+    if (mine && count != 1) many[__popc(others & before)] = lane;
+    if (lane == 0) {
+      n_lone = __popc(ones);
+      n_many = __popc(others);
+    }
   }
   __syncthreads();
   const int h0 = blockIdx.y * heads_per_cta, nh = min(heads_per_cta, a.heads - h0);
-  for (int idx = warp; idx < n_own * nh; idx += kWarps) {
-    const int e = own[idx / nh], h = h0 + idx % nh;
+  // The K and V tiles of the many, block by block and head by head, then the lone ones four heads at a time; what the latter
+  // leave over is done behind them.
+  const int tile_tasks = n_many * nh * 2, row_tasks = (nh + kRowHeads - 1) / kRowHeads, n_tasks = tile_tasks + n_lone * row_tasks;
+  for (int idx = warp; idx < n_tasks; idx += kWarps) {
+    int e, h, heads = 0;
+    uint32_t left;  // bit 2 k + v: the K (v = 0) or V tile of head h + k
+    if (idx < tile_tasks) {
+      e = many[(idx >> 1) / nh]; h = h0 + (idx >> 1) % nh;
+      left = 1u << (idx & 1);
+    } else {
+      const int i = idx - tile_tasks;
+      e = lone[i / row_tasks]; h = h0 + i % row_tasks * kRowHeads;
+      heads = min(kRowHeads, h0 + nh - h);
+    }
     const long long blk = block_of[e];
     const int m = lane < B ? member[e][lane] : -1;
     const uint32_t mask = __ballot_sync(0xffffffffu, m >= 0);
-    if (__popc(mask) == 1) {
+    if (heads > 0) {
       const int off = __ffs(mask) - 1;
-      if (fill_row<T, D, B>(a, blk, h, __shfl_sync(0xffffffffu, m, off), off, lane)) continue;
+      left = fill_rows<T, D, B>(a, blk, h, heads, __shfl_sync(0xffffffffu, m, off), off, lane);
     }
-#pragma unroll 1
-    for (int v = 0; v < 2; ++v)
-      fill_tile<T, D, B>((v ? a.value : a.key) + (size_t)h * D * sizeof(T), (size_t)(v ? a.value_stride : a.key_stride) * sizeof(T),
-                         (v ? a.vcache : a.kcache) + (size_t)blk * a.kbs + (size_t)h * a.khs,
-                         (v ? a.vscale : a.kscale) + (size_t)blk * a.sbs + (size_t)h * a.shs, member[e], mask, v == 1, lane);
+    for (; left; left &= left - 1) {
+      const int v = (__ffs(left) - 1) & 1, hh = h + ((__ffs(left) - 1) >> 1);
+      fill_tile<T, D, B>((v ? a.value : a.key) + (size_t)hh * D * sizeof(T), (size_t)(v ? a.value_stride : a.key_stride) * sizeof(T),
+                         (v ? a.vcache : a.kcache) + (size_t)blk * a.kbs + (size_t)hh * a.khs,
+                         (v ? a.vscale : a.kscale) + (size_t)blk * a.sbs + (size_t)hh * a.shs, member[e], mask, v == 1, lane);
+    }
   }
 }
 
-// A CTA: `win` (at most 64) consecutive entries of slot_mapping, cut into runs of consecutive slots inside 16 tokens of a block,
+// A CTA: `win` (at most kMaxWin) consecutive entries of slot_mapping, cut into runs of consecutive slots inside 16 tokens of a block,
 // and one head or a few. A warp takes the K or V rows of one (run, head) at a time. (V of a lone token costs the DRAM sectors
 // of the whole tile however it is read.)
-constexpr int kMaxWin = 64;
+constexpr int kMaxWin = 256;
 template <typename T, int D, int B>
 __global__ void __launch_bounds__(kWarps * 32) fp8_gather_kernel(const Fp8Rows a, const int win, const int heads_per_cta) {
   constexpr int kPasses = (D / 8 + 7) / 8;
@@ -535,7 +576,8 @@ cudaError_t launch_fill(const Fp8Rows& a, cudaStream_t s) {
 template <typename T, int D, int B>
 cudaError_t launch_gather(const Fp8Rows& a, cudaStream_t s) {
   // (short windows for few rows, long ones where runs are cut less often by them)
-  const int win = a.tokens * a.heads < (long long)sm_count() * 256 ? 16 : kMaxWin;
+  int win = kMaxWin;
+  while (win > 16 && a.tokens * a.heads < (long long)sm_count() * 4 * win) win /= 4;
   const unsigned windows = (unsigned)((a.tokens + win - 1) / win);
   const int hpc = heads_per_cta(windows, a.heads);
   return launch_kernel(fp8_gather_kernel<T, D, B>, dim3(windows, (unsigned)((a.heads + hpc - 1) / hpc)), kWarps * 32, 0, s, true, a, win, hpc);
