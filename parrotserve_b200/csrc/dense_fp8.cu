@@ -599,6 +599,7 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         // issuer without a tile in the last segment knows by it that the segment before that is over)
         if (!full_v(i)) { ok = false; break; }
         if (!split && more && !full_k(i + 1)) { ok = false; break; }
+        if (split && i + 1 < n && !pass_k(i + 1)) { ok = false; break; }  // the other issuer's; its slot is for the K after the next
         fence_proxy_async_smem();
         if (!wait_or_abort(bar(kBarP + x), tcx & 1, abort_flag, status)) { ok = false; break; }
         if (i == first && seg > 0 && !wait_or_abort(bar(kBarODrained + x), (seg - 1) & 1, abort_flag, status)) { ok = false; break; }
@@ -621,8 +622,7 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
         if (pair) ++turns;
         __syncwarp();
         if (split) {
-          // the tile behind it is the other issuer's; the K of the next one of this issuer comes into the slot of this tile
-          if (i + 1 < n && !pass_k(i + 1)) { ok = false; break; }
+          // the K of this issuer's next tile comes into the slot of this one
           if (more) {
             if (!full_k(i + 2)) { ok = false; break; }
             fence_proxy_async_smem();
