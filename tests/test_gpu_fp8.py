@@ -148,6 +148,25 @@ def test_fill_steps_grow_and_keep_scales():
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("tokens, heads, d, b", [(40, 7, 128, 16), (23, 5, 256, 32), (1030, 6, 64, 16)])
+def test_fill_lone_tokens_under_heads_that_differ(dtype, tokens, heads, d, b):
+    """One token for each block: some heads keep their scale, some grow it, some bring NaN, infinities or zeros."""
+    rng = np.random.default_rng(tokens + heads)
+    blocks = tokens + 4
+    cache = random_cache(rng, blocks, heads, d, b)
+    slots = rng.permutation(blocks)[:tokens] * b + rng.integers(0, b, size=tokens)
+    rows = []
+    for _ in range(2):
+        x = rng.standard_normal((tokens, heads, d)) * np.exp2(rng.integers(-4, 5, size=(tokens, heads, 1)))
+        x[rng.random((tokens, heads)) < 0.1] = 0
+        x[..., 3] = np.where(rng.random((tokens, heads)) < 0.05, np.nan, x[..., 3])
+        x[..., 40] = np.where(rng.random((tokens, heads)) < 0.05, np.inf, x[..., 40])
+        rows.append(torch.from_numpy(x).to(DEV).to(TYPES[dtype]))
+    got, want = fill_both(cache, *rows, slots)
+    same_cache(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 def test_fill_special_values(dtype):
     """NaN, infinities, zeros, the type's largest and smallest values, values between two codes, borders of a scale."""
     d = 64
@@ -209,6 +228,27 @@ def test_gather(dtype, d, b, heads):
         assert (got[~live] == left).all()
 
 
+@pytest.mark.parametrize("tokens, heads", [(700, 8), (6000, 8), (10000, 17)])
+def test_gather_of_runs(tokens, heads):
+    """Runs of consecutive slots of any length from any offset, with holes, up to sizes at which a CTA takes 256 of them."""
+    rng = np.random.default_rng(tokens)
+    blocks, b, d = 400, 32, 64
+    cache = random_cache(rng, blocks, heads, d, b)
+    slots = []
+    while len(slots) < tokens:
+        n, at = int(rng.integers(1, 90)), int(rng.integers(-5, blocks * b))
+        slots += [-1] if rng.random() < 0.1 else list(range(at, at + n))
+    slots = np.asarray(slots[:tokens])
+    key = torch.full((tokens, heads, d), 7.0, device=DEV, dtype=torch.bfloat16)
+    value = torch.full_like(key, -7.0)
+    pb.fp8_gather_cached_kv(key, value, *on_gpu(cache), torch.as_tensor(slots, device=DEV))
+    live = (slots >= 0) & (slots < blocks * b)
+    k, v = orc.token_rows(*cache, slots[live])
+    for got, want, left in ((key, k, 7.0), (value, v, -7.0)):
+        got = got.cpu()
+        assert torch.equal(got[live], torch.from_numpy(want).to(torch.bfloat16)) and (got[~live] == left).all()
+
+
 # ---------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------
@@ -238,6 +278,31 @@ def test_paged_attention(dtype, d, b, heads, kv):
     want = orc.attention(q.double().cpu().numpy(), cache, contexts, d ** -0.5, mapping)
     check_attention(out, want, dtype)
     assert (out[0] == 0).all()  # an empty context
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("d, b, heads, kv", [(64, 16, 8, 1), (128, 16, 6, 2), (128, 32, 2, 2), (256, 16, 1, 1), (96, 16, 3, 3)])
+def test_few_rows_with_many_partials(dtype, d, b, heads, kv):
+    """Long contexts beside short and empty ones, split into chunks over the chip. At most 128 terms of a chunk and 80 partials are
+    added one after another: 208 half steps of 2^-24, less than 2^-16, on top of what check_attention counts."""
+    rng = np.random.default_rng(d + heads)
+    lens = [9001, 0, 5, 4096]
+    cache, tables, q, mapping, contexts = paged_problem(rng, lens, heads, kv, d, b, dtype)
+    dev = on_gpu(cache)
+    m, l = torch.zeros(len(lens), heads, device=DEV), torch.zeros(len(lens), heads, device=DEV)
+    call = pb.Fp8AttentionCall(num_rows=len(lens), num_heads=heads, head_size=d, block_size=b, dtype=TYPES[dtype], device=torch.device(DEV),
+                               suffix_lens=i32(lens), suffix_tables=i32(tables), head_mapping=None if mapping is None else i32(mapping),
+                               suffix_chunk_blocks=128 // b)
+    out = torch.full_like(q, float("nan"))
+    call.run(q, out, *dev, m, l, _lib.PB_STATS_SAVE)
+    assert call.status() == 0
+    want = orc.attention(q.double().cpu().numpy(), cache, contexts, d ** -0.5, mapping)
+    check_attention(out, want, dtype, more=2.0 ** -16)
+    assert (out[1] == 0).all() and (l[1] == 0).all()
+    # and joined with what a call has left before: the same once more doubles the sums and keeps the mean
+    again = out.clone()
+    call.run(q, again, *dev, m, l, _lib.PB_STATS_LOAD_SAVE)
+    check_attention(again, want, dtype, more=2.0 ** -16 + torch.finfo(TYPES[dtype]).eps / 2)
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
