@@ -15,11 +15,16 @@
 //
 // Why: through mma.sync a (block, head) of 2 x 2 KiB costs a warp 64 conversions and 24 instructions of the fp16 pipe, some
 // 400 instructions in all, and 256 sequences of 1024 tokens x 32 heads ran at 4.1 TB/s, bound by their issue. Here four warps
-// spend about 100 instructions each on eight of them. What bounds it now is memory.
+// spend about 100 instructions each on eight of them: 315 us, 6.8 TB/s, memory is the bound. With several heads per item the bound is
+// the chain of a tile through its CTA (Q.K^T, weights, P.V: 2 us with four heads, 3 with eight): 128 sequences of 1024 tokens, 32
+// heads over 8, 59 us or 4.5 TB/s; one of 100000 tokens, 64 heads over 8, 65 us or 3.2 TB/s.
 //
-// Three CTAs an SM (two with more than four heads per item), so that the copies of one run under the chain of another.
-// Warps 0-3 softmax and epilogue, behind them one warp claims items and lists their tiles, two copy K
-// (one of them V too), one issues the MMAs and one makes the query operands. Every mbarrier wait is bounded; on expiry the CTA records a status, drains and returns.
+// Three CTAs an SM with one head per item, so that the copies of one run under the chain of another. With several, two, whose
+// heads are shared by two groups of softmax warps: the step from S to the weights is what the chain spends its time on (64 heads
+// over 8, 64 sequences of 2048 tokens 94 us with one group, 83 with two).
+// Warps 0-3 (and 4-7) softmax and epilogue, behind them one warp claims items and lists their tiles, two copy K (one of them V
+// too), one issues the MMAs and one makes the query operands. Every mbarrier wait is bounded; on expiry the CTA records a status,
+// drains and returns.
 #include <type_traits>
 
 #include "common.cuh"
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
     // S(t + 1) as soon as its tile is there, O(t) as soon as its weights are: whichever comes first.
     constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(C::kN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);  // fp32 += e4m3 . e4m3
     // Descriptors: the operands' addresses (in sixteens of bytes) are added to words made once. (Made anew for every MMA by the one
-    // thread that issues them they cost more than the products: 1500 cycles a tile with their polls, ISSUE_NOW so.)
+    // thread that issues them they cost more than the products, 1500 cycles a tile: 128 sequences of 32 heads over 8 took 88 us, 80 so.)
     const uint64_t dk = smem_desc(stage0, 2048, 128, 0), dv = smem_desc(stage0 + 8 * C::kTile, C::kTile, 128, 0);
     const uint64_t dq = smem_desc(smem_u32(smem + C::kOffQ), C::kN * 16, 128, 0), dw = smem_desc(smem_u32(smem + C::kOffW), C::kN * 16, 128, 0);
     const uint32_t k_hi = (uint32_t)(dk >> 32), v_hi = (uint32_t)(dv >> 32), n_hi = (uint32_t)(dq >> 32);

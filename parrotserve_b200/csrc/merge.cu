@@ -230,7 +230,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_rows_kernel(const Attn
 }
 
 // Few (row, head) pairs that may have many partials, of a long context split over all SMs: a CTA per pair, its warps share the
-// partials. (One row of 100003 tokens x 64 heads in 98 chunks: 62 us of a pair's sixteen lanes, WIDE_US so.)
+// partials. (One row of 100003 tokens x 64 heads in 98 chunks: 66 us of a pair's sixteen lanes, 26 so, most of them
+// under the kernel before.)
 constexpr int kWideWarps = 8, kWidePairs = 1024, kWideParts = 16;
 template <typename T, int D>
 __global__ void __launch_bounds__(kWideWarps * 32) merge_wide_kernel(const AttnDev d) {

