@@ -12,7 +12,7 @@
 // bytes inside a lane, then 4 x 4 words between four lanes) as 16 bytes a lane.
 //
 // Bound by memory where it is large: fill and gather of a batch with 16 prefills and 240 decodes (9.4k rows, 32 heads of 128, bf16)
-// 143 us, 3.4 TB/s of the 6.5 a copy reaches; what is lost lies in the latency of short CTAs and in the conversions of the gather.
+// 135 us, 3.6 TB/s of the 6.5 a copy reaches; what is lost lies in the latency of short CTAs and in the conversions of the gather.
 // Small calls are bound by latency: slots, scales and rows, store: 5 us each.
 //
 // Reference counterpart of the unquantised fill: reshape_and_cache_kernel (3rdparty/vllm/csrc/cache_kernels.cu:142-182).
@@ -344,10 +344,10 @@ __device__ __forceinline__ uint32_t fill_rows(const Fp8Rows& a, long long blk, i
   return left;
 }
 
-// CTAs an SM: two where the rows of a tile take 64 registers, three where they take fewer or are read twice. (Left to itself the
-// compiler takes up to 210 registers: 930 rows of fp32, heads of 80, blocks of 32, 41 us.)
+// CTAs an SM: four where the rows of a tile take 32 registers, two where they take 64, three where they are read twice. (Left to
+// itself the compiler takes up to 210 registers: 930 rows of fp32, heads of 80, blocks of 32, 41 us against 19.)
 template <typename T, int D, int B> constexpr int kRowWords = (B / 16) * ((D / 8 + 7) / 8) * 16 * (int)sizeof(T) / 2;
-template <typename T, int D, int B> constexpr int kFillCtas = kRowWords<T, D, B> > 32 && kRowWords<T, D, B> <= 64 ? 2 : 3;
+template <typename T, int D, int B> constexpr int kFillCtas = kRowWords<T, D, B> <= 32 ? 4 : kRowWords<T, D, B> <= 64 ? 2 : 3;
 
 // A CTA: 16 consecutive entries of slot_mapping, the blocks whose first token is among them, and one head or a few. A warp
 // takes one (block, head) at a time.
@@ -565,10 +565,11 @@ int fail(cudaError_t e) {
   return PB_ERR_LAUNCH;
 }
 
-// Heads per CTA, of `windows` windows: as many CTAs as keep the SMs busy, and what they share read as seldom as that allows.
+// Heads per CTA, of `windows` windows: as many CTAs as keep the SMs busy, and what they share read as seldom as that allows, up to
+// four (fill and gather of 9.4k rows x 32 heads, with at most 1 / 2 / 3 / 4 / 6 / 8 heads: 205 / 155 / 146 / 139 / 142 / 143 us).
 int heads_per_cta(long long windows, int heads) {
   const long long spare = windows * heads / ((long long)sm_count() * 8);
-  return (int)(spare < 1 ? 1 : spare > 8 ? 8 : spare);
+  return (int)(spare < 1 ? 1 : spare > 4 ? 4 : spare);
 }
 
 template <typename T, int D, int B>
