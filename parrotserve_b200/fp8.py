@@ -139,6 +139,7 @@ class Fp8AttentionCall(AttentionCall):
             raise _lib.PbError(_lib.PB_ERR_UNSUPPORTED, "Fp8AttentionCall", f"block_size={kwargs['block_size']}")
         with _on(torch.device(kwargs["device"]).index):
             super().__init__(**kwargs)
+        self._index = _one_device(*self._keep) if self._keep else None  # where the lengths and tables are
         self._cache = PbFp8Cache()
         self._cache_ref = C.byref(self._cache)
 
@@ -161,6 +162,8 @@ class Fp8AttentionCall(AttentionCall):
                   stats_mode=_lib.PB_STATS_NONE):
         p = self.params
         index = _one_device(query, out, key_cache, value_cache, key_scale, value_scale)
+        if self._index is not None and index != self._index:
+            raise RuntimeError("all tensors of a call must be on one device")
         hkv, d, b = _describe(self._cache, key_cache, value_cache, key_scale, value_scale)
         if query.dtype != self.dtype or out.dtype != self.dtype:
             raise RuntimeError("query and out must have the dtype of the call")
@@ -173,6 +176,11 @@ class Fp8AttentionCall(AttentionCall):
             raise RuntimeError("query/out must be dense over (head, dim)")
         if hkv != self._sized_for:
             self._size_for(hkv)
+        if stats_mode != _lib.PB_STATS_NONE:
+            for x in (qk_max, exp_sum):
+                if (x is None or x.dtype != torch.float32 or x.shape != self._q_shape[:2] or not x.is_contiguous()
+                        or x.get_device() != index):
+                    raise RuntimeError(f"qk_max and exp_sum must be float32 [{p.num_rows}, {p.num_heads}], contiguous, on the call's device")
         p.out, p.query = out.data_ptr(), query.data_ptr()
         p.q_stride, p.out_stride = qs[0], os[0]
         p.qk_max, p.exp_sum, p.stats_mode = _ptr(qk_max), _ptr(exp_sum), stats_mode

@@ -577,3 +577,14 @@ def test_operators_refuse():
         args = {**dict(query=row, out=torch.empty_like(row), key_cache=kc, value_cache=vc, key_scale=ks, value_scale=vs), **bad}
         with pytest.raises(RuntimeError):
             call.run(*args.values())
+
+
+def test_statistics_are_checked():
+    kc, vc, ks, vs = fp8.fp8_kv_cache(2, 2, 64, 16, DEV)
+    row = torch.zeros(3, 2, 64, dtype=torch.float16, device=DEV)
+    call = pb.Fp8AttentionCall(num_rows=3, num_heads=2, head_size=64, block_size=16, dtype=torch.float16, device=torch.device(DEV),
+                               suffix_lens=i32([1, 1, 1]), suffix_tables=i32([[0], [0], [0]]))
+    good = torch.zeros(3, 2, device=DEV)
+    for m, l in ((None, good), (good, None), (good.half(), good), (good, good[:2]), (good.cpu(), good), (good.t().contiguous().t(), good)):
+        with pytest.raises(RuntimeError):
+            call.run(row, torch.empty_like(row), kc, vc, ks, vs, m, l, _lib.PB_STATS_SAVE)
