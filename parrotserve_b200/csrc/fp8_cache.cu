@@ -627,6 +627,10 @@ int pb_fp8_reshape_and_cache(const pb_fp8_cache* cache, const void* key, const v
   pb::Fp8Rows a;
   const int rc = pb::bind_rows(cache, key, value, slot_mapping, slot_is_i64, num_tokens, key_stride, value_stride, dtype, &a);
   if (rc != PB_OK || num_tokens == 0) return rc;
+  // blocks or heads that share memory (a dimension of stride 0) would be written by several owners
+  if ((cache->num_blocks > 1 && (cache->kv_block_stride == 0 || cache->scale_block_stride == 0)) ||
+      (cache->num_kv_heads > 1 && cache->scale_head_stride == 0))
+    return PB_ERR_INVALID_ARG;
   const size_t need = pb_fp8_fill_workspace_bytes(num_tokens, cache->num_blocks, cache->block_size);
   if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < need)) return PB_ERR_WORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

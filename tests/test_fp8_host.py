@@ -70,6 +70,12 @@ def test_fill_needs_its_workspace():
     assert _lib.lib().pb_fp8_reshape_and_cache(C.byref(c), FAKE, FAKE, FAKE, 1, 0, 512, 512, _lib.PB_F16, None, 0, None) == _lib.PB_OK
 
 
+@pytest.mark.parametrize("over", [dict(kv_block_stride=0), dict(scale_block_stride=0), dict(scale_head_stride=0)])
+def test_fill_refuses_blocks_or_heads_that_share_memory(over):
+    c = cache(**over)
+    assert _lib.lib().pb_fp8_reshape_and_cache(C.byref(c), FAKE, FAKE, FAKE, 1, 3, 512, 512, _lib.PB_F16, None, 0, None) == _lib.PB_ERR_INVALID_ARG
+
+
 def attn_params(**over):
     p = _lib.PbAttnParams(out=FAKE, query=FAKE, scale=0.1, dtype=_lib.PB_F16, num_rows=2, num_heads=4, num_kv_heads=4, head_size=128,
                           block_size=16, q_stride=512, out_stride=512, suffix_lens=FAKE, suffix_tables=FAKE, suffix_table_stride=2)
