@@ -463,6 +463,8 @@ int pb_fp8_gather_cached_kv(const pb_fp8_cache* cache, void* key, void* value, c
  * brings them), num_kv_heads, head_size and block_size have to be the cache's, and it brings no new tokens
  * (slot_mapping, key_new and value_new are NULL: the fill is a call of its own). p->dtype is the type of query and out.
  * Lists planned by one family of entry points are not valid for the other.
+ * A (row, head) that sees a token is NaN if its query holds a NaN or an infinity, or a token's K a NaN, in every shape and however the
+ * work is split; so are the sums that such a call saves, and what a later call makes of them.
  * The workspace has pb_fp8_attn_workspace_bytes(p) bytes; head_mapping and num_kv_heads are read for it besides what
  * pb_attn_workspace_bytes reads (a head mapping need only be NULL or not).
  */

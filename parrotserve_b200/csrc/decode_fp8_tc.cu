@@ -36,6 +36,7 @@ namespace {
 
 using namespace dense;
 using fp8::kMinLv;
+using fp8::told_max;
 using fp8::warp_max;
 
 constexpr int kDescSlots = 8, kItemSlots = 4;  // (how far the lister runs ahead: it waits for three loads in a row per item)
@@ -552,9 +553,9 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
 #pragma unroll
       for (int h = 0; h < N; ++h) {
         if (h0 + h < hpi) {
-          const float m = max4(ctl.left_max[g][at][h]), ref_h = ctl.left_ref[g][at][h];
           const float4 sums = ctl.left_sum[g][at][h];
           const float sum = (sums.x + sums.y) + (sums.z + sums.w);
+          const float m = told_max(max4(ctl.left_max[g][at][h]), sum), ref_h = ctl.left_ref[g][at][h];
           const float fix = ref_h == -INFINITY ? 0.f : fast_exp2(ref_h - m);
           const float v = join_parts<N>(o, h);
           const size_t slot = partial_slot(d, row, part, head + h0 + h);

@@ -31,6 +31,7 @@ namespace {
 
 using namespace dense;
 using fp8::kMinLv;
+using fp8::told_max;
 using fp8::warp_max;
 
 constexpr float kShift = 7.f;                            // w <= 2^(kTau + kShift) = 2^15
@@ -765,6 +766,7 @@ dense_fp8_kernel(const AttnDev d, const __grid_constant__ CUtensorMap pmap, cons
           st.m_run = m;
         }
       }
+      st.m_true = told_max(st.m_true, st.l_run);
       const int nrows_x = min(128, it.nrows - (pair ? x * 128 : 0));
       const bool row_ok = r < nrows_x;
       const int row = it.row0 + qrow;

@@ -39,6 +39,10 @@ __device__ __forceinline__ float scale_for(float top) {
   return __uint_as_float((uint32_t)(e < 1 ? 1 : e) << 23);
 }
 
+// The maximum m that a partial carries. Maxima drop NaN; a partial whose logits are all NaN would go to the merge with -inf, like one without
+// tokens, and be left out. One whose sum l is NaN (a logit was) carries 0 then, and its NaN enters the sums whatever the others' maxima are.
+__device__ __forceinline__ float told_max(float m, float l) { return l == l ? m : 0.f; }
+
 // Maximum over a warp (NaN counts as nothing, like fmaxf).
 __device__ __forceinline__ float warp_max(float v) {
   float m;

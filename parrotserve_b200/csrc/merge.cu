@@ -84,7 +84,10 @@ __device__ __forceinline__ void merge_one(const AttnDev& d, const int row, const
   if (load_prev && active) {
     m_prev = d.qk_max[idx];
     l_prev = d.exp_sum[idx];
-    if (!(l_prev > 0.f)) { l_prev = 0.f; m_prev = -INFINITY; }
+    if (!(l_prev > 0.f)) {
+      if (!(d.key_scale && l_prev != l_prev)) l_prev = 0.f;  // (8-bit calls: an earlier partial of NaN stays NaN)
+      m_prev = -INFINITY;
+    }
   }
 
   // pass 1: global maximum (lane j of the pair reads the statistics of partial j; with at most
@@ -144,7 +147,7 @@ __device__ __forceinline__ void merge_one(const AttnDev& d, const int row, const
   }
 #pragma unroll
   for (int o = kPairLanes / 2; o >= 1; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-  if (!active || (parts.direct && !poison)) return;
+  if (!active || (parts.direct && !poison)) return;  // (no call with statistics has rows finished before)
   if (l_prev > 0.f) {
     const float w = fast_exp2(m_prev - M) * l_prev;
     L += w;
@@ -160,7 +163,7 @@ __device__ __forceinline__ void merge_one(const AttnDev& d, const int row, const
       }
     }
   }
-  const float inv = poison ? __int_as_float(0x7fc00000) : (L > 0.f) ? 1.f / L : 0.f;
+  const float inv = (poison || l_prev != l_prev) ? __int_as_float(0x7fc00000) : (L > 0.f) ? 1.f / L : 0.f;
   T* op = reinterpret_cast<T*>(d.out) + (size_t)row * d.out_stride + (size_t)head * D;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
@@ -174,7 +177,7 @@ __device__ __forceinline__ void merge_one(const AttnDev& d, const int row, const
   }
   if ((d.stats_mode & PB_STATS_SAVE) && sub == 0) {
     d.qk_max[idx] = M;
-    d.exp_sum[idx] = L;
+    d.exp_sum[idx] = l_prev != l_prev ? l_prev : L;
   }
 }
 
@@ -258,7 +261,10 @@ __global__ void __launch_bounds__(kWideWarps * 32) merge_wide_kernel(const AttnD
   if (d.stats_mode & PB_STATS_LOAD) {
     m_prev = d.qk_max[idx];
     l_prev = d.exp_sum[idx];
-    if (!(l_prev > 0.f)) { l_prev = 0.f; m_prev = -INFINITY; }
+    if (!(l_prev > 0.f)) {
+      if (l_prev == l_prev) l_prev = 0.f;  // (an earlier partial of NaN stays NaN)
+      m_prev = -INFINITY;
+    }
   }
   float M = m_prev;
   for (int j = tid; j < n; j += kThreads) M = fmaxf(M, d.ml[slot_of(j)].x);
@@ -319,7 +325,7 @@ __global__ void __launch_bounds__(kWideWarps * 32) merge_wide_kernel(const AttnD
   for (int w = 0; w < kWideWarps; ++w) L += red_l[w];
   const float w_prev = l_prev > 0.f ? fast_exp2(m_prev - M) * l_prev : 0.f;
   L += w_prev;
-  const float inv = poison ? __int_as_float(0x7fc00000) : (L > 0.f) ? 1.f / L : 0.f;
+  const float inv = (poison || l_prev != l_prev) ? __int_as_float(0x7fc00000) : (L > 0.f) ? 1.f / L : 0.f;
   T* op = reinterpret_cast<T*>(d.out) + (size_t)row * d.out_stride + (size_t)head * D;
   for (int i = tid; i < D; i += kThreads) {
     float v = 0.f;
@@ -330,7 +336,7 @@ __global__ void __launch_bounds__(kWideWarps * 32) merge_wide_kernel(const AttnD
   }
   if ((d.stats_mode & PB_STATS_SAVE) && tid == 0) {
     d.qk_max[idx] = M;
-    d.exp_sum[idx] = L;
+    d.exp_sum[idx] = l_prev != l_prev ? l_prev : L;
   }
 }
 

@@ -372,19 +372,24 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
         const int qrow = MULTI ? g : 0;
         const bool live = MULTI ? g < hpi : g < 2;
         const T* qs = reinterpret_cast<const T*>(stage + 2 * C::kTileBytes) + (live ? qrow : 0) * D + 4 * t;
-        float top = 0.f;
+        float top = 0.f, odd = 0.f;  // odd: NaN if the row holds NaN or an infinity, whose products could all be -inf
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           float f[4];
           load_q4<T>(qs + c * 16, f);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(f[i]));
+          for (int i = 0; i < 4; ++i) {
+            top = fmaxf(top, fabsf(f[i]));
+            odd = fmaf(f[i], 0.f, odd);
+          }
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+        odd += __shfl_xor_sync(0xffffffffu, odd, 2);
         const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
         const float up = __uint_as_float((uint32_t)(267 - e) << 23);
-        mul = d.scale_log2e * __uint_as_float((uint32_t)(e - 13) << 23);
+        mul = d.scale_log2e * __uint_as_float((uint32_t)(e - 13) << 23) + odd;
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           float f[4];
@@ -487,10 +492,11 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
       __syncwarp();  // stage s may be overwritten from here on
       if (mt.w & 512) {  // last block of the item: the partial, re-based on the exact maximum
         const int it_row = mt.x, it_head = mt.y & 0xffff, it_part = mt.y >> 16;
-        const float fix = ref == -INFINITY ? 0.f : fast_exp2(ref - kTop - m_run);
         float l = l_run;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
+        m_run = fp8::told_max(m_run, l);
+        const float fix = ref == -INFINITY ? 0.f : fast_exp2(ref - kTop - m_run);
         if constexpr (MULTI) {
           const float f0 = __shfl_sync(0xffffffffu, fix, 8 * t), f1 = __shfl_sync(0xffffffffu, fix, 8 * t + 4);
 #pragma unroll
