@@ -439,7 +439,7 @@ typedef struct pb_fp8_cache {
  *   old   = 0 if offset 0 of the block is among the new tokens (the block begins anew), else its scale
  *   scale = max(old, need); new cells = e4m3(x / scale), to nearest even; NaN and infinities are stored as NaN
  *   the block's other cells are re-quantised, e4m3(c * old / scale), only when the scale grew (exact but for values that
- *   leave the normal range of e4m3, as long as both scales are powers of two)
+ *   leave the normal range of e4m3, as long as both scales are powers of two; of a tile whose scale was 0 they become 0)
  * Tokens of a block may stand anywhere in slot_mapping; of tokens with the same slot the last in the list counts. A
  * negative slot, or one outside the cache, skips its token. Rows are fp32, fp16 or bf16 (dtype). Blocks and heads of the cache
  * and its scales may not share memory (strides of 0 are refused).

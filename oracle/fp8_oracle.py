@@ -63,7 +63,9 @@ def fill(key_codes, value_codes, key_scale, value_scale, key, value, slots) -> N
                 now = max(old, scale_for(float(finite.max())))
                 inv = np.float32(1.0) / np.float32(now) if now > 0 else np.float32(0.0)
                 out = tile.copy()
-                if 0.0 < old < now:
+                if old == 0.0 and now > 0.0 and 0 not in members:
+                    out = np.zeros_like(tile)  # a tile with scale 0 is zero, whatever its codes
+                elif 0.0 < old < now:
                     with np.errstate(all="ignore"):
                         out = to_codes((VALUES[tile].astype(np.float32) * np.float32(old)) * inv)
                 for off, t in members.items():

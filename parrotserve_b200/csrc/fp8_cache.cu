@@ -157,8 +157,9 @@ __device__ __forceinline__ void rows_to_tokens(const uint4 (&row)[2], uint2 (&to
 constexpr int kWarps = 8;
 constexpr int kScanTokens = 1024;  // (the table's kernel is a launch more: 5 us)
 
-// Codes that a block holds already, under its grown scale.
+// Codes that a block holds already, under its grown scale. (Under a scale of 0 they all stood for 0, whatever they are.)
 __device__ __forceinline__ uint32_t requantised(uint32_t w, float held, float inv) {
+  if (held == 0.f) return 0u;
   const float2 a = fp8::to_float2(w), b = fp8::to_float2(w >> 16);
   return fp8::pack4(fp8::scaled(__fmul_rn(a.x, held), inv), fp8::scaled(__fmul_rn(a.y, held), inv),
                     fp8::scaled(__fmul_rn(b.x, held), inv), fp8::scaled(__fmul_rn(b.y, held), inv));
@@ -227,7 +228,7 @@ __device__ __forceinline__ void fill_tile(const uint8_t* rows, size_t row_bytes,
   }
   const float now = fmaxf(held, fp8::scale_for(top));
   const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
-  const bool grown = held > 0.f && now > held;
+  const bool grown = !(mask & 1u) && now > held;
 #pragma unroll
   for (int sub = 0; sub < kSubs; ++sub) {
     const uint32_t sub_mask = (mask >> (16 * sub)) & 0xffffu;
@@ -316,7 +317,7 @@ __device__ __forceinline__ uint32_t fill_rows(const Fp8Rows& a, long long blk, i
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) top = __uint_as_float(max(__float_as_uint(top), __shfl_xor_sync(0xffffffffu, __float_as_uint(top), o)));
     const float now = fmaxf(held[h], fp8::scale_for(top));
-    if (__any_sync(0xffffffffu, !is_finite(top) || (held[h] > 0.f && now > held[h]))) {
+    if (__any_sync(0xffffffffu, !is_finite(top) || (off != 0 && now > held[h]))) {
       left |= 3u << (2 * h);
       continue;
     }
