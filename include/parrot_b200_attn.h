@@ -414,7 +414,7 @@ int pb_sample_top_p_host_settings(const void* logits, int32_t dtype, int32_t num
  * each block and kv head: an element stands for code * scale. Layout as for the other types, with x = 16:
  *   K: [num_blocks, num_kv_heads, head_size/16, block_size, 16]   V: [num_blocks, num_kv_heads, head_size, block_size]
  *   scales: [num_blocks, num_kv_heads] fp32, strides in elements, the same for key_scale and value_scale.
- * Scales are >= 0; 0 says that the whole tile is zero. Head sizes 64, 80, 96, 112, 128, 256; block sizes 16 and 32.
+ * Scales are >= 0; 0 says that the whole tile is zero (its codes may be any but NaN where a context reaches). Head sizes 64, 80, 96, 112, 128, 256; block sizes 16 and 32.
  * Strides of the caches count elements, which are bytes here, and are multiples of 16.
  */
 typedef struct pb_fp8_cache {
@@ -435,7 +435,8 @@ typedef struct pb_fp8_cache {
 /*
  * KV fill into the 8-bit cache: pb_reshape_and_cache that quantises. For every block b that receives tokens, and every
  * head, K and V each on their own:
- *   need  = the smallest power of two with max |x| <= 448 * need over the new tokens' finite elements (0 for all zero)
+ *   need  = the smallest power of two from 2^-126 on with max |x| <= 448 * need over the new tokens' finite elements (0 if all elements
+ *           are zero; 2^-126 if all finite ones are and there are others)
  *   old   = 0 if offset 0 of the block is among the new tokens (the block begins anew), else its scale
  *   scale = max(old, need); new cells = e4m3(x / scale), to nearest even; NaN and infinities are stored as NaN
  *   the block's other cells are re-quantised, e4m3(c * old / scale), only when the scale grew (exact but for values that

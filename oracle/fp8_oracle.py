@@ -60,7 +60,10 @@ def fill(key_codes, value_codes, key_scale, value_scale, key, value, slots) -> N
                 new = np.stack([rows[t, head] for t in members.values()])
                 finite = np.where(np.isfinite(new), np.abs(new), 0.0)
                 old = 0.0 if 0 in members else float(scales[blk, head])
-                now = max(old, scale_for(float(finite.max())))
+                top = float(finite.max())
+                if not np.isfinite(new).all():
+                    top = max(top, math.ldexp(1.0, -126))  # a tile with scale 0 is zero, which NaN is not
+                now = max(old, scale_for(top))
                 inv = np.float32(1.0) / np.float32(now) if now > 0 else np.float32(0.0)
                 out = tile.copy()
                 if old == 0.0 and now > 0.0 and 0 not in members:

@@ -60,3 +60,30 @@ def test_tokens_of_zeros_then_others(dtype):
     key, value = torch.empty_like(rows[0]), torch.empty_like(rows[1])
     pb.fp8_gather_cached_kv(key, value, *dev, torch.tensor(slots, device=DEV))
     assert not key[:2].any() and not value[:2].any() and key[2:].any() and value[2:].any()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_nan_beside_zeros_has_a_scale(dtype, tokens):
+    """A tile whose only finite elements are zeros, with a NaN or an infinity among them: gather, decode and a shared prefix all see
+    NaN where it stands, and zeros elsewhere."""
+    heads, d, b, rows = 2, 128, 16, 5
+    cache = tuple(np.zeros_like(x) for x in random_cache(np.random.default_rng(1), 4, heads, d, b))
+    key = torch.zeros(tokens, heads, d, dtype=TYPES[dtype], device=DEV)
+    value = torch.zeros_like(key)
+    value[tokens - 1, 0, 9], value[0, 1, 100], key[0, 1, 3] = float("inf"), float("nan"), float("nan")
+    slots = [2 * b + i for i in range(tokens)]
+    got, want = fill_both(cache, key, value, slots)
+    same_cache(got, want)
+    assert got[3][2].tolist() == [2.0 ** -126] * 2 and got[2][2].tolist() == [0.0, 2.0 ** -126]
+    dev = on_gpu(got)
+    k, v = torch.ones_like(key), torch.ones_like(value)
+    pb.fp8_gather_cached_kv(k, v, *dev, torch.tensor(slots, device=DEV))
+    for x, rows_in in ((k, key), (v, value)):
+        assert torch.equal(x.isnan(), ~rows_in.isfinite()) and not torch.nan_to_num(x, nan=0).any()
+    q = rand_rows(np.random.default_rng(2), rows, heads, d, dtype)
+    lens, tables = i32([tokens] * rows), i32([[2]] * rows)
+    for out in (pb.fp8_paged_attention(q, *dev, None, lens, tables),
+                pb.fp8_flash_paged_attention(q, *dev, None, tokens, i32([2]), i32([0] * rows), i32([[0]] * rows))):
+        assert torch.equal(out[:, 0].isnan(), torch.arange(d, device=DEV).eq(9).expand(rows, d))
+        assert not torch.nan_to_num(out[:, 0], nan=0).any() and out[:, 1].isnan().all()
