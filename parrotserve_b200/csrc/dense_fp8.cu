@@ -223,7 +223,7 @@ __device__ __forceinline__ void list_tiles(const AttnDev& d, SegmentWalker& walk
       if (ti == i) {
         const float lv = cur.vs > 0.f ? fmaxf(__log2f(cur.vs), kMinLv) : cur.vs == 0.f ? kMinLv : __int_as_float(0x7fc00000);
         e.blk[j] = cur.vs == 0.f ? ~cur.blk : cur.blk;  // (the complement: its V is zero)
-        e.ks[j] = cur.ks == 0.f ? 1e-30f : cur.ks;  // (a logit of -inf times 0 would be NaN)
+        e.ks[j] = cur.ks;
         e.lv[j] = lv;
         e.inv[j] = fast_exp2(-lv);
         if (j == 0) {

@@ -1,0 +1,52 @@
+"""Value and key scales of the 8-bit cache over the range that a fill can make, from 2^-126 on, and their spread inside a row."""
+import numpy as np
+import pytest
+import torch
+
+import parrotserve_b200 as pb
+from oracle import fp8_oracle as orc
+from tests.test_gpu_fp8 import DEV, TYPES, i32, on_gpu, paged_problem
+
+pytestmark = pytest.mark.gpu
+
+
+def check(out, want, dtype, unit=0, far=False):
+    """The tolerance of check_attention (its derivation is there) without its absolute terms, of an output multiplied by 2^-unit. Instead:
+    * what falls below the normal numbers: half the smallest step of the output's type (bf16 2^-134, fp32 2^-150), and of fp32 for each
+      of at most 128 partials of a row before they are divided by their sum (>= 1);
+    * far: exponents of value scales beyond 2^6 are fp32 numbers below 2^8. The kernel for fp32 queries adds three of them in a row (half
+      steps of 2^-17) and takes a logarithm with an error of 2^-22 of itself, 2^-15: together less than 2^-14 of a weight."""
+    e = torch.finfo(TYPES[dtype]).eps / 2
+    weights, logits = (2.0 ** -22, 2.0 ** -19) if dtype == "f32" else (2.0 ** -11, 2.0 ** -17 + 2.0 ** -19)
+    small = (128 + (1 if dtype == "f32" else 2.0 ** 16)) * np.ldexp(1.0, -150 - unit)
+    got = np.ldexp(out.detach().double().cpu().numpy(), -unit)
+    assert np.isfinite(got).all()
+    more = 2.0 ** -14 if far and dtype == "f32" else 0.0
+    tol = e * np.abs(want.out) + (2 * weights + 2 * logits * want.reach[..., None] + 2.0 ** -20 + more) * want.absolute + 2.0 ** -30 * want.loud + small
+    worst = (np.abs(got - want.out) / tol)[want.absolute > 0].max(initial=0.0)
+    assert worst <= 1.0, f"{worst:.3g} of the tolerance"
+    assert not got[want.absolute == 0].any()
+
+
+SHAPES = [("bf16", 128, 16, 2, 2), ("bf16", 64, 16, 8, 2), ("bf16", 96, 16, 8, 1), ("f32", 128, 16, 2, 2), ("f32", 80, 32, 6, 2), ("bf16", 128, 32, 3, 3)]
+
+
+@pytest.mark.parametrize("dtype, d, b, heads, kv", SHAPES)
+def test_a_key_scale_of_zero_is_zero(dtype, d, b, heads, kv):
+    """Logits of exactly 0 under key scales of 0, whatever the codes and however large the queries: the mean of the values."""
+    rng = np.random.default_rng(d)
+    lens = [40, 300]
+    cache, tables, q, mapping, contexts = paged_problem(rng, lens, heads, kv, d, b, dtype)
+    cache[2][:] = 0.0
+    want = orc.attention(np.zeros(q.shape), cache, contexts, d ** -0.5, mapping)
+    out = pb.fp8_paged_attention(q * 1e30, *on_gpu(cache), None if mapping is None else i32(mapping), i32(lens), i32(tables))
+    check(out, want, dtype)
+    if dtype == "bf16" and b == 16 and d == 128:
+        rows = [lens[0]] * 70  # and by the prefix kernel
+        big = q[:1].expand(70, -1, -1).contiguous() * 1e30
+        call = pb.Fp8AttentionCall(num_rows=70, num_heads=heads, head_size=d, block_size=b, dtype=TYPES[dtype], device=torch.device(DEV),
+                                   group_row_offsets=i32([0, 70]), group_prefix_lens=i32([lens[1]]), group_tables=i32(tables[1:]),
+                                   suffix_lens=i32([0] * 70), suffix_tables=i32(np.zeros((70, 1))))
+        got = call.run(big, torch.empty_like(big), *on_gpu(cache))
+        many = orc.attention(np.zeros(big.shape), cache, [contexts[1]] * len(rows), d ** -0.5, mapping)
+        check(got, many, dtype)
