@@ -44,6 +44,8 @@ __device__ __forceinline__ float scale_for(float top) {
 // tokens, and be left out. One whose sum l is NaN (a logit was) carries 0 then, and its NaN enters the sums whatever the others' maxima are.
 __device__ __forceinline__ float told_max(float m, float l) { return l == l ? m : 0.f; }
 
+__device__ __forceinline__ float pow2(float e) { return __uint_as_float((uint32_t)((int)e + 127) << 23); }  // whole e in [-126, 127]
+
 // Maximum over a warp (NaN counts as nothing, like fmaxf).
 __device__ __forceinline__ float warp_max(float v) {
   float m;

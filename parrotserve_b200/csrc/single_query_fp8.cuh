@@ -496,33 +496,36 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, 1) sq8_attn_kernel(const Att
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         m_run = fp8::told_max(m_run, l);
-        const float fix = ref == -INFINITY ? 0.f : fast_exp2(ref - kTop - m_run);
+        // 2^(ref - kTop - m), in two factors: by value scales near 2^-126 or 2^120 one would leave the range of fp32
+        const float fix_e = ref == -INFINITY ? 0.f : fminf(fmaxf(rintf(0.5f * (ref - kTop - m_run)), -126.f), 126.f);
+        const float fix = ref == -INFINITY ? 0.f : fast_exp2(ref - kTop - m_run - fix_e), fix2 = fp8::pow2(fix_e);
         if constexpr (MULTI) {
           const float f0 = __shfl_sync(0xffffffffu, fix, 8 * t), f1 = __shfl_sync(0xffffffffu, fix, 8 * t + 4);
+          const float p0 = __shfl_sync(0xffffffffu, fix2, 8 * t), p1 = __shfl_sync(0xffffffffu, fix2, 8 * t + 4);
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int hh = 2 * t + c;
             if (hh < hpi) {
               float* ap = d.acc + partial_slot(d, it_row, it_part, it_head + hh) * D + g;
-              const float f = c ? f1 : f0;
+              const float f = c ? f1 : f0, p = c ? p1 : p0;
 #pragma unroll
               for (int j = 0; j < kSteps; ++j) {
-                ap[16 * j] = oacc[j][c] * f;
-                ap[16 * j + 8] = oacc[j][2 + c] * f;
+                ap[16 * j] = oacc[j][c] * f * p;
+                ap[16 * j + 8] = oacc[j][2 + c] * f * p;
               }
             }
           }
           if (t == 0 && g < hpi) d.ml[partial_slot(d, it_row, it_part, it_head + g)] = make_float2(m_run, l);
         } else {
           const size_t slot = partial_slot(d, it_row, it_part, it_head);
-          const float f0 = __shfl_sync(0xffffffffu, fix, 0);
+          const float f0 = __shfl_sync(0xffffffffu, fix, 0), p0 = __shfl_sync(0xffffffffu, fix2, 0);
           float* ap = d.acc + slot * D + g;
 #pragma unroll
           for (int j = 0; j < kSteps; ++j) {
             const float lo = oacc[j][0] + oacc[j][1], hi = oacc[j][2] + oacc[j][3];
             if (t == 0) {
-              ap[16 * j] = lo * f0;
-              ap[16 * j + 8] = hi * f0;
+              ap[16 * j] = lo * f0 * p0;
+              ap[16 * j + 8] = hi * f0 * p0;
             }
           }
           if (lane == 0) d.ml[slot] = make_float2(m_run, l);

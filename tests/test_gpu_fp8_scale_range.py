@@ -31,6 +31,19 @@ def check(out, want, dtype, unit=0, far=False):
 SHAPES = [("bf16", 128, 16, 2, 2), ("bf16", 64, 16, 8, 2), ("bf16", 96, 16, 8, 1), ("f32", 128, 16, 2, 2), ("f32", 80, 32, 6, 2), ("bf16", 128, 32, 3, 3)]
 
 
+@pytest.mark.parametrize("shift", [-115, -100, -92, -70, -25, 40, 100])
+@pytest.mark.parametrize("dtype, d, b, heads, kv", [s for s in SHAPES if s[0] == "f32" or s[2] == 32])
+def test_decodes_with_value_scales_of_any_size(dtype, d, b, heads, kv, shift):
+    rng = np.random.default_rng(d + heads)
+    lens = [1, 17, 0, 300, 700]
+    cache, tables, q, mapping, contexts = paged_problem(rng, lens, heads, kv, d, b, dtype)
+    cache[3][:] = np.ldexp(cache[3], shift)
+    scales = np.ldexp(cache[3], -shift)
+    want = orc.attention(q.double().cpu().numpy(), (*cache[:3], scales), contexts, d ** -0.5, mapping)
+    out = pb.fp8_paged_attention(q, *on_gpu(cache), None if mapping is None else i32(mapping), i32(lens), i32(tables))
+    check(out, want, dtype, shift, far=True)
+
+
 @pytest.mark.parametrize("dtype, d, b, heads, kv", SHAPES)
 def test_a_key_scale_of_zero_is_zero(dtype, d, b, heads, kv):
     """Logits of exactly 0 under key scales of 0, whatever the codes and however large the queries: the mean of the values."""
