@@ -305,7 +305,7 @@ __global__ void __launch_bounds__((DecCfg<D, HMAX>::kThreads), (DecCfg<D, HMAX>:
         if (lane < 8) {
           e.blk[lane] = blk;
           e.ks[lane] = k1;
-          e.lv[lane] = v1 > 0.f ? fmaxf(__log2f(v1), kMinLv) : v1 == 0.f ? -INFINITY : __int_as_float(0x7fc00000);
+          e.lv[lane] = v1 >= fp8::kMinValueScale ? __log2f(v1) : v1 >= 0.f ? -INFINITY : __int_as_float(0x7fc00000);
         }
         if (lane == 0) {
           e.nb = nb;

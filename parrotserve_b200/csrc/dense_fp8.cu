@@ -3,8 +3,8 @@
 // What the scales do. With (ks, vs) the scales of block b, c = scale * log2(e) and f the factor of the query row (below):
 //     lg_t = s_t * ks[b] * c / f         u_t = lg_t + lv[b],  lv = log2(vs)
 //     w_t  = 2^(u_t - M + kShift)        l += 2^-lv[b] * sum of the block's w_t          O += w_t v8_t
-// with M the lazy reference of max u, so that the weights use fp16's range whatever the scales are. A block with vs = 0 gets
-// zeros as V and counts with lv = kMinLv, and scales below 2^kMinLv count as that: what l loses there is below 2^-26 of it.
+// with M the lazy reference of max u, so that the weights use fp16's range whatever the scales are. A block with vs = 0, or below 2^kMinLv,
+// which counts as 0, gets zeros as V and lv = kMinLv.
 //
 // What feeds the tensor cores:
 //   S_x = Q_x . K^T   kind::f8f6f4 on the codes of K as they are. Q comes as a sum of e4m3 parts, each the rounded remainder of
@@ -221,8 +221,9 @@ __device__ __forceinline__ void list_tiles(const AttnDev& d, SegmentWalker& walk
       if (tc >= kDescSlots && !wait_or_abort(ring->empty_bar(tc), ring->parity(tc) ^ 1, abort_flag, status)) { ok = false; break; }
       TileDesc& e = ring->desc[tc % kDescSlots];
       if (ti == i) {
-        const float lv = cur.vs > 0.f ? fmaxf(__log2f(cur.vs), kMinLv) : cur.vs == 0.f ? kMinLv : __int_as_float(0x7fc00000);
-        e.blk[j] = cur.vs == 0.f ? ~cur.blk : cur.blk;  // (the complement: its V is zero)
+        const bool none = cur.vs >= 0.f && cur.vs < fp8::kMinValueScale;
+        const float lv = none ? kMinLv : cur.vs > 0.f ? __log2f(cur.vs) : __int_as_float(0x7fc00000);
+        e.blk[j] = none ? ~cur.blk : cur.blk;  // (the complement: its V is zero)
         e.ks[j] = cur.ks;
         e.lv[j] = lv;
         e.inv[j] = fast_exp2(-lv);

@@ -8,7 +8,10 @@
 namespace pb {
 namespace fp8 {
 
-constexpr float kMinLv = -100.f;  // log2 of the smallest value scale told apart from smaller ones by the tensor-core kernels
+// The tensor-core kernels hold sums of 2^-lv with lv = log2 of the value scales, so these have bounds: below 2^kMinLv they count as 0 (the
+// values are below 4e-28, the type's 2^-126 is out of reach of the sums), and from 2^100 on small weights are lost from the sums. (A unit
+// chosen by an item's first blocks would lift both; its one vote among the listing warp's lanes cost the prefix kernel 3 %.)
+constexpr float kMinLv = -100.f, kMinValueScale = 7.888609052210118e-31f;
 
 // Two codes (the low 16 bits of `w`) as fp16, exactly: every e4m3 value, subnormals included, is a normal fp16 value.
 __device__ __forceinline__ uint32_t to_half2(uint32_t w) {

@@ -7,8 +7,8 @@ Keys and values are e4m3 codes in the framework's paged layout (``x = 16``) with
 * block sizes 16 and 32, head sizes 64, 80, 96, 112, 128, 256; queries and rows in fp16, bf16 or fp32.
 
 The operators stand beside those of ``ops`` and take the four cache tensors where those take two. What is filled with
-``fp8_reshape_and_cache`` has powers of two as scales; attention and gather take any scales >= 0 (a tile with scale 0 is zero and holds no
-NaN). Nothing here falls back
+``fp8_reshape_and_cache`` has powers of two as scales; attention and gather take others too (a tile with scale 0 is zero and holds no
+NaN; attention of 16-bit queries counts value scales below 2^-100 as 0 and is inexact above 2^100). Nothing here falls back
 to torch: the operators fail without the library or a GPU.
 
 Beside the reference's ``vllm_reshape_and_cache`` (kernels/vllm/reshape_and_cache.py:9-22) and ``flash_paged_attention``

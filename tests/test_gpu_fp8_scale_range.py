@@ -5,9 +5,15 @@ import torch
 
 import parrotserve_b200 as pb
 from oracle import fp8_oracle as orc
-from tests.test_gpu_fp8 import DEV, TYPES, i32, on_gpu, paged_problem
+from tests.test_gpu_fp8 import DEV, TYPES, i32, layer_problem, on_gpu, paged_problem
 
 pytestmark = pytest.mark.gpu
+
+
+def counted(cache, dtype, d, b):
+    """The cache as attention reads it: on the tensor cores (16-bit queries, blocks of 16) value scales below 2^-100 are 0."""
+    tensor_cores = dtype != "f32" and b == 16 and d in (64, 96, 128)
+    return (*cache[:3], np.where(cache[3] < 2.0 ** -100, 0, cache[3]) if tensor_cores else cache[3])
 
 
 def check(out, want, dtype, unit=0, far=False):
@@ -32,16 +38,65 @@ SHAPES = [("bf16", 128, 16, 2, 2), ("bf16", 64, 16, 8, 2), ("bf16", 96, 16, 8, 1
 
 
 @pytest.mark.parametrize("shift", [-115, -100, -92, -70, -25, 40, 100])
-@pytest.mark.parametrize("dtype, d, b, heads, kv", [s for s in SHAPES if s[0] == "f32" or s[2] == 32])
+@pytest.mark.parametrize("dtype, d, b, heads, kv", SHAPES)
 def test_decodes_with_value_scales_of_any_size(dtype, d, b, heads, kv, shift):
     rng = np.random.default_rng(d + heads)
     lens = [1, 17, 0, 300, 700]
     cache, tables, q, mapping, contexts = paged_problem(rng, lens, heads, kv, d, b, dtype)
     cache[3][:] = np.ldexp(cache[3], shift)
-    scales = np.ldexp(cache[3], -shift)
+    scales = np.ldexp(counted(cache, dtype, d, b)[3], -shift)
     want = orc.attention(q.double().cpu().numpy(), (*cache[:3], scales), contexts, d ** -0.5, mapping)
     out = pb.fp8_paged_attention(q, *on_gpu(cache), None if mapping is None else i32(mapping), i32(lens), i32(tables))
     check(out, want, dtype, shift, far=True)
+
+
+@pytest.mark.parametrize("shift", [-110, -92, -70, 40, 100])
+@pytest.mark.parametrize("dtype, spec", [
+    ("bf16", dict(heads=2, kv=2, prefixes=(515,), group_rows=(70,), suffixes=tuple(range(1, 71)))),            # a lone row tile
+    ("bf16", dict(heads=3, kv=3, prefixes=(1500, 3000, 130), group_rows=(7, 140, 5), suffixes=tuple([3] * 152))),  # and pairs
+    ("bf16", dict(heads=2, kv=2, segments=((130, 0), (300, 5), (20, 0)))),                                      # finished rows
+    ("bf16", dict(heads=4, kv=1, segments=((300, 500), (140, 900)), suffixes=(30, 0))),
+    ("f32", dict(heads=2, kv=2, prefixes=(100,), group_rows=(5,), suffixes=(1, 16, 17, 40, 300))),
+])
+def test_layers_with_value_scales_of_any_size(dtype, spec, shift):
+    rng = np.random.default_rng(7)
+    call, q, cache, contexts, mapping = layer_problem(rng, dtype=dtype, **spec)
+    cache[3][:] = np.ldexp(cache[3], shift)
+    scales = np.ldexp(counted(cache, dtype, 128, 16)[3], -shift)
+    want = orc.attention(q.double().cpu().numpy(), (*cache[:3], scales), contexts, q.shape[2] ** -0.5, mapping)
+    check(call.run(q, torch.empty_like(q), *on_gpu(cache)), want, dtype, shift, far=True)
+    assert call.status() == 0
+
+
+@pytest.mark.parametrize("first, then", [(-126, -60), (-60, -126), (-10, 60), (60, -10), (-100, -30), (100, 30), (-80, -80), (0, -75)])
+@pytest.mark.parametrize("dtype, d, b, heads, kv", SHAPES)
+def test_value_scales_that_differ_inside_a_row(dtype, d, b, heads, kv, first, then):
+    """Scales near 2^first in the first 40 blocks of a context and near 2^then behind them, in one item of 64 blocks."""
+    rng = np.random.default_rng((d + heads + first) % 1000)
+    lens = [700 * b // 16, 1000 * b // 16]
+    cache, tables, q, mapping, contexts = paged_problem(rng, lens, heads, kv, d, b, dtype)
+    lift = np.full(cache[3].shape[0], then)
+    lift[tables[:, :40].ravel()] = first
+    cache[3][:] = np.ldexp(np.ones(cache[3].shape), np.maximum(lift[:, None] + rng.integers(-3, 4, size=cache[3].shape), -126)).astype(np.float32)
+    want = orc.attention(q.double().cpu().numpy(), counted(cache, dtype, d, b), contexts, d ** -0.5, mapping)
+    call = pb.Fp8AttentionCall(num_rows=2, num_heads=heads, head_size=d, block_size=b, dtype=TYPES[dtype], device=torch.device(DEV),
+                               suffix_lens=i32(lens), suffix_tables=i32(tables), head_mapping=None if mapping is None else i32(mapping),
+                               suffix_chunk_blocks=64)
+    out = call.run(q, torch.empty_like(q), *on_gpu(cache))
+    assert call.status() == 0
+    check(out, want, dtype, far=True)
+
+
+@pytest.mark.parametrize("first, then", [(-120, -60), (-60, -110), (-10, 60), (60, -10), (0, -75)])
+def test_value_scales_that_differ_under_a_prefix(first, then):
+    """The same for a prefix and its rows' own contexts: shares of the prefix begin anywhere in it."""
+    rng = np.random.default_rng(9)
+    call, q, cache, contexts, mapping = layer_problem(rng, dtype="bf16", heads=2, kv=2, prefixes=(3000,), group_rows=(9,), suffixes=tuple([40] * 9))
+    lift = np.full(cache[3].shape[0], then)
+    lift[contexts[0][:1500] // 16] = first
+    cache[3][:] = np.ldexp(np.ones(cache[3].shape), np.maximum(lift[:, None] + rng.integers(-3, 4, size=cache[3].shape), -126)).astype(np.float32)
+    want = orc.attention(q.double().cpu().numpy(), counted(cache, "bf16", 128, 16), contexts, 128 ** -0.5, mapping)
+    check(call.run(q, torch.empty_like(q), *on_gpu(cache)), want, "bf16", far=True)
 
 
 @pytest.mark.parametrize("dtype, d, b, heads, kv", SHAPES)
