@@ -438,7 +438,7 @@ typedef struct pb_fp8_cache {
  * KV fill into the 8-bit cache: pb_reshape_and_cache that quantises. For every block b that receives tokens, and every
  * head, K and V each on their own:
  *   need  = the smallest power of two from 2^-126 on with max |x| <= 448 * need over the new tokens' finite elements (0 if all elements
- *           are zero; 2^-126 if all finite ones are and there are others)
+ *           are zero; at least 2^-100 if one is NaN or infinite)
  *   old   = 0 if offset 0 of the block is among the new tokens (the block begins anew), else its scale
  *   scale = max(old, need); new cells = e4m3(x / scale), to nearest even; NaN and infinities are stored as NaN
  *   the block's other cells are re-quantised, e4m3(c * old / scale), only when the scale grew (exact but for values that

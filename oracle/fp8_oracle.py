@@ -62,7 +62,7 @@ def fill(key_codes, value_codes, key_scale, value_scale, key, value, slots) -> N
                 old = 0.0 if 0 in members else float(scales[blk, head])
                 top = float(finite.max())
                 if not np.isfinite(new).all():
-                    top = max(top, math.ldexp(1.0, -126))  # a tile with scale 0 is zero, which NaN is not
+                    top = max(top, math.ldexp(448.0, -100))  # tiles with smaller scales may be read as zeros, which NaN is not
                 now = max(old, scale_for(top))
                 inv = np.float32(1.0) / np.float32(now) if now > 0 else np.float32(0.0)
                 out = tile.copy()

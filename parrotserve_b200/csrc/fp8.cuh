@@ -34,7 +34,6 @@ __device__ __forceinline__ uint32_t pack2(__half2 v) {
 }
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return pack2(a, b) | (pack2(c, d) << 16); }
 
-constexpr float kMinScale = 1.17549435e-38f;  // 2^-126, the smallest scale but 0
 // The smallest power of two s with top <= 448 * s (448 = 1.75 * 2^8), from 2^-126 on; 0 for 0. top is finite, >= 0.
 __device__ __forceinline__ float scale_for(float top) {
   if (!(top > 0.f)) return 0.f;

@@ -225,7 +225,7 @@ __device__ __forceinline__ void fill_tile(const uint8_t* rows, size_t row_bytes,
     }
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    top = fmaxf(top, fp8::kMinScale);  // (a tile with scale 0 is zero, which NaN is not)
+    top = fmaxf(top, 448.f * fp8::kMinValueScale);  // (tiles with smaller scales may be read as zeros, which NaN is not)
   }
   const float now = fmaxf(held, fp8::scale_for(top));
   const float inv = now > 0.f ? __frcp_rn(now) : 0.f;

@@ -75,7 +75,7 @@ def test_nan_beside_zeros_has_a_scale(dtype, tokens):
     slots = [2 * b + i for i in range(tokens)]
     got, want = fill_both(cache, key, value, slots)
     same_cache(got, want)
-    assert got[3][2].tolist() == [2.0 ** -126] * 2 and got[2][2].tolist() == [0.0, 2.0 ** -126]
+    assert got[3][2].tolist() == [2.0 ** -100] * 2 and got[2][2].tolist() == [0.0, 2.0 ** -100]
     dev = on_gpu(got)
     k, v = torch.ones_like(key), torch.ones_like(value)
     pb.fp8_gather_cached_kv(k, v, *dev, torch.tensor(slots, device=DEV))
@@ -87,3 +87,29 @@ def test_nan_beside_zeros_has_a_scale(dtype, tokens):
                 pb.fp8_flash_paged_attention(q, *dev, None, tokens, i32([2]), i32([0] * rows), i32([[0]] * rows))):
         assert torch.equal(out[:, 0].isnan(), torch.arange(d, device=DEV).eq(9).expand(rows, d))
         assert not torch.nan_to_num(out[:, 0], nan=0).any() and out[:, 1].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_nan_beside_tiny_values_has_a_scale(dtype):
+    """NaN that joins tiny values, with them and after them, is not read as zero either."""
+    heads, d, b, rows = 1, 128, 16, 5
+    rng = np.random.default_rng(6)
+    cache = tuple(np.zeros_like(x) for x in random_cache(rng, 4, heads, d, b))
+    tiny = rand_rows(rng, 4, heads, d, dtype, 2.0 ** -120)
+    tiny[1, 0, 5] = float("nan")
+    late = tiny[1:2].clone()
+    for steps in ([(0, 4)], [(0, 1), (2, 2), (3, 1)]):
+        dev, want = on_gpu(cache), tuple(x.copy() for x in cache)
+        at = 0
+        for first, n in steps:
+            new = late if (first, n) == (3, 1) else tiny[first:first + n].contiguous()
+            slots = list(range(2 * b + at, 2 * b + at + len(new)))
+            at += len(new)
+            pb.fp8_reshape_and_cache(tiny[:len(new)].abs().nan_to_num().contiguous(), new, *dev, torch.tensor(slots, device=DEV))
+            orc.fill(*want, tiny[:len(new)].abs().nan_to_num().double().cpu().numpy(), new.double().cpu().numpy(), slots)
+            same_cache(to_host(dev), want)
+        assert want[3][2, 0] == 2.0 ** -100
+        q = rand_rows(rng, rows, heads, d, dtype)
+        for out in (pb.fp8_paged_attention(q, *dev, None, i32([at] * rows), i32([[2]] * rows)),
+                    pb.fp8_flash_paged_attention(q, *dev, None, at, i32([2]), i32([0] * rows), i32([[0]] * rows))):
+            assert torch.equal(out[:, 0].isnan(), torch.arange(d, device=DEV).eq(5).expand(rows, d))
