@@ -56,6 +56,19 @@ __global__ void __launch_bounds__(256) fp8_link_kernel(const Fp8Rows a, const in
   }
 }
 
+// Rows and cells are read with ordinary loads: these kernels begin while the one before them may still write what they read, which the
+// read-only path does not allow. (In this form, so that stores to other places do not hold them up.)
+__device__ __forceinline__ uint4 load16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 load8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
 // Eight consecutive elements of a row, as they come.
 template <typename T> struct Raw8 {
   static constexpr int kVecs = sizeof(T) / 2;
@@ -66,7 +79,7 @@ template <typename T> struct Raw8 {
   }
   __device__ __forceinline__ void load(const uint8_t* p) {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < kVecs; ++i) v[i] = load16(p + 16 * i);
   }
   __device__ __forceinline__ void floats(float* f) const {
 #pragma unroll
@@ -504,7 +517,7 @@ __global__ void __launch_bounds__(kWarps * 32) fp8_gather_kernel(const Fp8Rows a
           const int c = p * 8 + dg, i = 4 * g + j;
           tok[p][j] = make_uint2(0u, 0u);
           if (c < D / 8 && i >= off0 && i < off0 + len)
-            tok[p][j] = __ldg(reinterpret_cast<const uint2*>(tile + ((c >> 1) * B + sub * 16 + i) * 16 + 8 * (c & 1)));
+            tok[p][j] = load8(tile + ((c >> 1) * B + sub * 16 + i) * 16 + 8 * (c & 1));
         }
     } else {
       uint4 row[kPasses][2];
@@ -514,7 +527,7 @@ __global__ void __launch_bounds__(kWarps * 32) fp8_gather_kernel(const Fp8Rows a
         for (int k = 0; k < 2; ++k) {
           const int c = p * 8 + dg;
           row[p][k] = make_uint4(0u, 0u, 0u, 0u);
-          if (c < D / 8) row[p][k] = __ldg(reinterpret_cast<const uint4*>(tile + (c * 8 + 2 * g + k) * B + sub * 16));
+          if (c < D / 8) row[p][k] = load16(tile + (c * 8 + 2 * g + k) * B + sub * 16);
         }
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) rows_to_tokens(row[p], tok[p], g);
