@@ -494,7 +494,8 @@ int pb_fp8_attention(const pb_attn_params* p, const pb_fp8_cache* cache, void* s
  *   rows behind the last token: slot -1, position 0, suffix length 0.
  * row_offsets [num_requests + 1]: first row of every request (its first num_prefills + 1 entries are seg_row_offsets);
  * kv_lens [num_requests]: tokens held afterwards (the first num_prefills entries are seg_kv_lens);
- * *free_head_out: entries of free_blocks taken so far. Only block_tables is changed in place, so the call can be repeated.
+ * *free_head_out: entries of free_blocks taken so far. Only block_tables is changed in place, so the call can be repeated. Results and
+ * workspace share no memory with the inputs nor with each other (kv_lens is not context_lens, free_head_out not free_head: refused).
  * suffix_tables may be NULL. Negative lengths count as 0. workspace: pb_block_tables_workspace_bytes(num_requests) bytes, 0
  * for up to a thousand requests.
  */

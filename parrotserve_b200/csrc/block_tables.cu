@@ -243,6 +243,21 @@ int pb_build_block_tables(const int32_t* context_lens, const int32_t* new_lens, 
   if (num_requests > 1 && table_stride < table_width) return PB_ERR_INVALID_ARG;
   const size_t need = pb_block_tables_workspace_bytes(num_requests);
   if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < need)) return PB_ERR_WORKSPACE;
+  // Every CTA reads the inputs for itself while others write results: no result may lie on an input, nor on another result.
+  const int64_t r = num_requests, t = num_tokens;
+  const struct { const void* p; int64_t bytes; } spans[] = {
+      // results, the workspace among them
+      {block_tables, r > 0 && table_width > 0 ? 4 * ((r - 1) * table_stride + table_width) : 0}, {slot_mapping, 8 * t}, {positions, 8 * t},
+      {row_offsets, 4 * (r + 1)}, {kv_lens, 4 * r}, {suffix_lens, 4 * t}, {suffix_tables, 4 * t * table_width}, {free_head_out, 4},
+      {num_failed, 4}, {workspace, (int64_t)need},
+      // inputs
+      {context_lens, 4 * r}, {new_lens, 4 * r}, {free_blocks, 4 * (int64_t)num_free}, {free_head, 4}, {prefix_lens, 4 * r}};
+  constexpr int kResults = 10, kSpans = sizeof(spans) / sizeof(spans[0]);
+  for (int i = 0; i < kResults; ++i)
+    for (int j = i + 1; j < kSpans; ++j) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(spans[i].p), b = reinterpret_cast<uintptr_t>(spans[j].p);
+      if (a && b && spans[i].bytes > 0 && spans[j].bytes > 0 && a < b + spans[j].bytes && b < a + spans[i].bytes) return PB_ERR_INVALID_ARG;
+    }
   pb::TablesDev d;
   d.context_lens = context_lens; d.new_lens = new_lens; d.block_tables = block_tables; d.free_blocks = free_blocks;
   d.free_head = free_head; d.prefix_lens = prefix_lens;
