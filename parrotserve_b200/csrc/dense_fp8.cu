@@ -321,7 +321,7 @@ __device__ __forceinline__ void copy_k_and_q(const AttnDev& d, int lane, uint32_
     const int s = tc & 1;
     if (!wait_or_abort(ring->full_bar(tc), ring->parity(tc), abort_flag, status, 50)) break;
     const TileDesc& e = ring->desc[tc % kDescSlots];
-    const int nb = e.nb;
+    const int nb = e.nb, nrows = e.nrows, row0 = e.row0, head = e.head;  // (read before K is let go: the slot is written anew behind its products)
     if (nb == 0) break;
     if (!wait_or_abort(bar(kBarEmptyK + s), ((tc >> 1) & 1) ^ 1, abort_flag, status, 50)) break;
     for (int j = 0; j < nb; ++j) {
@@ -332,8 +332,8 @@ __device__ __forceinline__ void copy_k_and_q(const AttnDev& d, int lane, uint32_
       for (int k = 0; k < 4; ++k) cp_async16(dst + k * 2 * (kTileBlocks * 256), src + k * 512);
     }
     cp_async_arrive_noinc(bar(kBarFullK + s));
-    if (e.nrows > 0) {
-      const int nsub = e.nrows > 128 ? 2 : 1, row0 = e.row0, head = e.head;
+    if (nrows > 0) {
+      const int nsub = nrows > 128 ? 2 : 1;
       bool ok = true;
       for (int x = 0; x < nsub && ok; ++x) {
         if (segx[x] > 0 && !wait_or_abort(bar(kBarQFree + x), (segx[x] - 1) & 1, abort_flag, status, 50)) { ok = false; break; }
