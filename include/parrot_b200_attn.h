@@ -468,6 +468,8 @@ int pb_fp8_gather_cached_kv(const pb_fp8_cache* cache, void* key, void* value, c
  * Lists planned by one family of entry points are not valid for the other.
  * A (row, head) that sees a token is NaN if its query holds a NaN or an infinity, or a token's K a NaN, in every shape and however the
  * work is split; so are the sums that such a call saves, and what a later call makes of them.
+ * A NaN in V is one in its element of the rows that see the token. In a causal segment on the tensor cores, which take 256 rows and 128
+ * tokens at a time, it may reach that element of the segment's earlier rows too (0 times NaN), as with the 16-bit caches.
  * The workspace has pb_fp8_attn_workspace_bytes(p) bytes; head_mapping and num_kv_heads are read for it besides what
  * pb_attn_workspace_bytes reads (a head mapping need only be NULL or not).
  */

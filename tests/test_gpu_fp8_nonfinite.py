@@ -135,3 +135,38 @@ def test_key_codes_of_layers(case):
         for r in range(rows):
             where[r, :heads // kv] |= s in contexts[r]
     same_but(call.run(q, torch.empty_like(q), *on_gpu(cache)), clean, where)
+
+
+@pytest.mark.parametrize("case", range(len(LAYERS)))
+@pytest.mark.parametrize("where_in", [0.0, 0.4, 1.0])
+def test_value_codes_of_layers(case, where_in):
+    """A NaN code in V: NaN in its element for the rows that see the token. The tensor cores take 256 rows of a prompt with 128 tokens at a
+    time: earlier rows of the prompt may get NaN in that element too, if a row of their 256 sees one of the token's 128 (0 times NaN).
+    Nothing else changes."""
+    dtype, spec = LAYERS[case]
+    rng = np.random.default_rng(90 + case)
+    call, q, cache, contexts, _ = layer_problem(rng, dtype=dtype, **spec)
+    rows, heads, d = q.shape
+    b, kv = cache[1].shape[3], cache[1].shape[1]
+    clean = call.run(q, torch.empty_like(q), *on_gpu(cache)).clone()
+    where, may = np.zeros((rows, heads, d), dtype=bool), np.zeros((rows, heads, d), dtype=bool)
+    at = np.concatenate([[0], np.cumsum([n for n, _ in spec.get("segments", ())])])
+    for row, element, head in ((rows // 2, d - 3, 0), (rows - 1, 34, kv - 1)):
+        s = int(contexts[row][int(where_in * (len(contexts[row]) - 1))])
+        cache[1][s // b, head, element, s % b] = 0xFF
+        under = slice(head * (heads // kv), (head + 1) * (heads // kv))
+        for r in range(rows):
+            if s in contexts[r]:
+                where[r, under, element] = True
+        for lo, hi, (n, past) in zip(at, at[1:], spec.get("segments", ())):
+            own = contexts[hi - 1][-(n + past):]  # the prompt's own tokens, behind a prefix
+            if s in own:
+                tile = int(np.flatnonzero(own == s)[0]) // 128 * 128
+                for first in range(0, n, 256):
+                    last = min(n, first + 256)
+                    if tile < past + last:
+                        may[lo + first:lo + last, under, element] = True
+    got = call.run(q, torch.empty_like(q), *on_gpu(cache))
+    assert call.status() == 0
+    leaked = torch.as_tensor(may & ~where, device=DEV) & got.isnan()
+    same_but(torch.where(leaked, clean, got), clean, where)
