@@ -161,7 +161,7 @@ template <int N> __device__ __forceinline__ float join_parts(const uint32_t* c, 
   return sum;
 }
 
-// One claimed item as the lister keeps it; `id` < 0: none.
+// One claimed item as the lister keeps it (live == false: none).
 struct DecClaim {
   int row, head, kvh, part, nblk, ntok, table_kind, tbl_off;
   int bid[4];
@@ -744,7 +744,7 @@ cudaError_t launch_dec_t(const AttnDev& d, int head_size, cudaStream_t s) {
 }  // namespace
 
 bool decode_fp8_supported(int dtype, int head_size, int block_size) {
-  return (dtype == PB_F16 || dtype == PB_BF16) && block_size == 16 && (head_size == 64 || head_size == 96 || head_size == 128);
+  return fp8::decode_on_tc(dtype == PB_F16 || dtype == PB_BF16, head_size, block_size);
 }
 cudaError_t launch_decode_fp8(const AttnDev& d, int dtype, int head_size, cudaStream_t s) {
   return dtype == PB_F16 ? launch_dec_t<__half>(d, head_size, s) : launch_dec_t<__nv_bfloat16>(d, head_size, s);

@@ -13,6 +13,11 @@ namespace fp8 {
 // chosen by an item's first blocks would lift both; its one vote among the listing warp's lanes cost the prefix kernel 3 %.)
 constexpr float kMinLv = -100.f, kMinValueScale = 7.888609052210118e-31f;
 
+// The shapes whose single queries go to the tcgen05 kernel (decode_fp8_tc.cu); the others go to single_query_fp8.cuh.
+constexpr bool decode_on_tc(bool half_queries, int head_size, int block_size) {
+  return half_queries && block_size == 16 && (head_size == 64 || head_size == 96 || head_size == 128);
+}
+
 // Two codes (the low 16 bits of `w`) as fp16, exactly: every e4m3 value, subnormals included, is a normal fp16 value.
 __device__ __forceinline__ uint32_t to_half2(uint32_t w) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);

@@ -563,12 +563,16 @@ cudaError_t launch_sq8(const AttnDev& d, cudaStream_t s) {
   return launch_kernel(kfn, d.num_sms, (WARPS + 1) * 32, smem, s, true, d);
 }
 
-// All head and block sizes of one type of queries.
+template <typename T, int D, int B>
+cudaError_t launch_sq8_shape(const AttnDev& d, cudaStream_t s) {
+  if constexpr (fp8::decode_on_tc(sizeof(T) == 2, D, B)) return cudaErrorInvalidValue;  // (never asked for here)
+  else return d.gqa_heads > 1 ? launch_sq8<T, D, B, true>(d, s) : launch_sq8<T, D, B, false>(d, s);
+}
+// All head and block sizes of one type of queries that the tcgen05 kernel does not take.
 template <typename T>
 cudaError_t launch_sq8_all(const AttnDev& d, int head_size, int block_size, cudaStream_t s) {
-#define PB_SQ8(DD)                                                                                                       \
-  if (head_size == DD && block_size == 16) return d.gqa_heads > 1 ? launch_sq8<T, DD, 16, true>(d, s) : launch_sq8<T, DD, 16, false>(d, s); \
-  if (head_size == DD && block_size == 32) return d.gqa_heads > 1 ? launch_sq8<T, DD, 32, true>(d, s) : launch_sq8<T, DD, 32, false>(d, s);
+#define PB_SQ8(DD) \
+  if (head_size == DD) return block_size == 16 ? launch_sq8_shape<T, DD, 16>(d, s) : launch_sq8_shape<T, DD, 32>(d, s);
   PB_SQ8(64) PB_SQ8(80) PB_SQ8(96) PB_SQ8(112) PB_SQ8(128) PB_SQ8(256)
 #undef PB_SQ8
   return cudaErrorInvalidValue;
