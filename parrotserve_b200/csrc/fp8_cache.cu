@@ -360,7 +360,9 @@ __device__ __forceinline__ uint32_t fill_rows(const Fp8Rows& a, long long blk, i
 }
 
 // CTAs an SM: four where the rows of a tile take 32 registers, two where they take 64, three where they are read twice. (Left to
-// itself the compiler takes up to 210 registers: 930 rows of fp32, heads of 80, blocks of 32, 41 us against 19.)
+// itself the compiler takes up to 210 registers: 930 rows of fp32, heads of 80, blocks of 32, 41 us against 19. The bounds spill: 24 to 40
+// bytes a thread in 16-bit tiles of 16 tokens x 80 to 128 and of 32 x 64, as much in fp32 ones of 16 x 64 and 32 x 80 to 112, 120 to 128 in fp32
+// of 256. They were chosen by time, the other bounds of a shape were not tried one by one.)
 template <typename T, int D, int B> constexpr int kRowWords = (B / 16) * ((D / 8 + 7) / 8) * 16 * (int)sizeof(T) / 2;
 template <typename T, int D, int B> constexpr int kFillCtas = kRowWords<T, D, B> <= 32 ? 4 : kRowWords<T, D, B> <= 64 ? 2 : 3;
 
