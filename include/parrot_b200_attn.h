@@ -414,7 +414,8 @@ int pb_sample_top_p_host_settings(const void* logits, int32_t dtype, int32_t num
  * each block and kv head: an element stands for code * scale. Layout as for the other types, with x = 16:
  *   K: [num_blocks, num_kv_heads, head_size/16, block_size, 16]   V: [num_blocks, num_kv_heads, head_size, block_size]
  *   scales: [num_blocks, num_kv_heads] fp32, strides in elements, the same for key_scale and value_scale.
- * Scales are >= 0; 0 says that the whole tile is zero (its codes may be any but NaN where a context reaches). Head sizes 64, 80, 96, 112, 128, 256; block sizes 16 and 32.
+ * Scales are >= 0; 0 says that the whole tile is zero (its codes may be any but NaN where a context reaches). Head sizes
+ * 64, 80, 96, 112, 128, 256; block sizes 16 and 32.
  * Attention of 16-bit queries counts value scales below 2^-100 as 0 where a context is read on the tensor cores (blocks of 16; head sizes
  * 64, 96 and 128 for single queries, 128 for prefixes and segments); above 2^100 it loses weights below 2^-26 from its sums.
  * Strides of the caches count elements, which are bytes here, and are multiples of 16.

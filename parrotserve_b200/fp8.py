@@ -102,9 +102,11 @@ def fp8_reshape_and_cache(key, value, key_cache, value_cache, key_scale, value_s
     int64 slot per token, negative: none) and updates the scales.
 
     The scale of a (block, head) becomes the largest of what it was and the smallest power of two with which the new
-    tokens' largest element fits (448 codes); when it grows the tokens that the block holds already are re-quantised. A
+    tokens' largest element fits (448 codes); when it grows the tokens that the block holds already are re-quantised (under a scale
+    of 0 they were zeros and stay so). A
     call that brings the token at offset 0 of a block begins the block anew: what it held, its scale included, is void. Tokens of
-    a block may stand in any order; of tokens with one slot the last counts. NaN and infinities are cached as NaN."""
+    a block may stand in any order; of tokens with one slot the last counts. NaN and infinities are cached as NaN, under a scale of at least
+    2^-100."""
     c, t, index, (_slots, *args) = _rows(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping)
     if t == 0:
         return
