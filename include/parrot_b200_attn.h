@@ -446,7 +446,7 @@ typedef struct pb_fp8_cache {
  *   leave the normal range of e4m3, as long as both scales are powers of two; of a tile whose scale was 0 they become 0)
  * Tokens of a block may stand anywhere in slot_mapping; of tokens with the same slot the last in the list counts. A
  * negative slot, or one outside the cache, skips its token. Rows are fp32, fp16 or bf16 (dtype). Blocks and heads of the cache
- * and its scales may not share memory (strides of 0 are refused).
+ * and its scales may not share memory (strides under which they would are refused).
  * workspace: pb_fp8_fill_workspace_bytes(num_tokens, num_blocks, block_size) bytes of scratch, contents irrelevant; none (0) for
  * few tokens.
  */

@@ -577,6 +577,16 @@ int bind_rows(const pb_fp8_cache* c, const void* key, const void* value, const v
   return PB_OK;
 }
 
+// Whether the tiles of a [blocks, heads] grid lie apart: neighbours by the smaller stride, and their rows by the larger one. (Grids whose
+// rows interleave without a collision are not looked for: no view of a cache is one.)
+bool lie_apart(int64_t blocks, int64_t block_stride, int64_t heads, int64_t head_stride, int64_t tile) {
+  if (blocks <= 1) return heads <= 1 || head_stride >= tile;
+  if (heads <= 1) return block_stride >= tile;
+  const bool heads_inside = head_stride <= block_stride;
+  const int64_t inner = heads_inside ? head_stride : block_stride, count = heads_inside ? heads : blocks;
+  return inner >= tile && (heads_inside ? block_stride : head_stride) >= (count - 1) * inner + tile;
+}
+
 int fail(cudaError_t e) {
   set_cuda_error(e);
   return PB_ERR_LAUNCH;
@@ -644,9 +654,9 @@ int pb_fp8_reshape_and_cache(const pb_fp8_cache* cache, const void* key, const v
   pb::Fp8Rows a;
   const int rc = pb::bind_rows(cache, key, value, slot_mapping, slot_is_i64, num_tokens, key_stride, value_stride, dtype, &a);
   if (rc != PB_OK || num_tokens == 0) return rc;
-  // blocks or heads that share memory (a dimension of stride 0) would be written by several owners
-  if ((cache->num_blocks > 1 && (cache->kv_block_stride == 0 || cache->scale_block_stride == 0)) ||
-      (cache->num_kv_heads > 1 && cache->scale_head_stride == 0))
+  // blocks or heads that share memory would be written by several owners
+  if (!pb::lie_apart(cache->num_blocks, cache->kv_block_stride, cache->num_kv_heads, cache->kv_head_stride, (int64_t)cache->head_size * cache->block_size) ||
+      !pb::lie_apart(cache->num_blocks, cache->scale_block_stride, cache->num_kv_heads, cache->scale_head_stride, 1))
     return PB_ERR_INVALID_ARG;
   const size_t need = pb_fp8_fill_workspace_bytes(num_tokens, cache->num_blocks, cache->block_size);
   if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < need)) return PB_ERR_WORKSPACE;
